@@ -73,8 +73,9 @@ const char* nyion_version(void);
 /* Range report of the current device.  Kernels that carry an input in a
  * narrower format than the reference's f32 record, in a per-device sticky
  * word, when an input does not fit it: prefill's V (binary16 in the P.V
- * product: |v| >= 65520 or infinite) and the q of decode over binary16 or
- * Q4-20B pools (binary16 high part: |q| >= 65520).  This call orders itself after the work on
+ * product: |v| >= 65520 or infinite), the q of decode over binary16 or
+ * Q4-20B pools (binary16 high part: |q| >= 65520) and the rows written to an
+ * 8-bit cache (infinite or NaN).  This call orders itself after the work on
  * `stream`, waits for it, takes (reads and clears) the word and returns
  * NYION_OK, or NYION_ERR_RANGE with nyion_last_error() naming what
  * overflowed since the last take.  The word is per device, not per stream:
@@ -572,6 +573,137 @@ int nyion_q4_dequant(const uint8_t* in, int64_t n_rows, int head_dim, float* out
                      nyion_stream_t stream);
 int nyion_q4_quantize(const float* in, int64_t n_rows, int head_dim, uint8_t* out,
                       nyion_stream_t stream);
+
+/* ------------------------------------ batched serving on an 8-bit cache */
+
+/* No counterpart in the reference, which serves one sequence at a time from
+ * f32 and Q4-20B pages (swamp-engine/src/cache.rs).  A step of a batch is
+ * three calls, none of which needs the host to know a length exactly:
+ *   nyion_batch_map             lengths -> slots, positions, new pages;
+ *   nyion_kv8_write             each layer's new K/V rows -> the 8-bit cache;
+ *   nyion_kv8_decode_attention  one query row per sequence.
+ *
+ * The cache holds K and V codes [num_blocks][n_kv_heads][block_tokens]
+ * [head_dim], one byte each, and one f32 scale per (block, kv head) for each
+ * of K and V, [num_blocks][n_kv_heads]; a value is its code's value times the
+ * scale of its block and head.  Codes are e4m3 (the OCP format: 4 exponent
+ * bits, 3 mantissa bits, largest value 448) or 8-bit integers (-127..127).
+ * block_tokens is 16, 32, 64, 128 or 256, head_dim 64 or 128; codes are
+ * 16-byte and scales 4-byte aligned.  Live rows hold finite codes and
+ * positive finite scales, as nyion_kv8_write leaves them; what blocks hold
+ * behind a sequence's last token is never used, whatever it is. */
+enum nyion_kv8_code { NYION_KV8_E4M3 = 0, NYION_KV8_INT8 = 1 };
+
+/* Element type of the K/V rows that are written and of q and out. */
+enum nyion_io_dtype { NYION_IO_F32 = 0, NYION_IO_BF16 = 1 };
+
+typedef struct nyion_kv8_cache {
+    uint8_t* k_codes;
+    uint8_t* v_codes;
+    float*   k_scales;
+    float*   v_scales;
+    int32_t  num_blocks;
+    int32_t  n_kv_heads;
+    int32_t  block_tokens;
+    int32_t  head_dim;
+    int32_t  code;     /* nyion_kv8_code */
+    int32_t  reserved; /* 0 */
+} nyion_kv8_cache;
+
+/* What happens to a score between q.k and the softmax.  For query position i
+ * and key position j, in this order:
+ *   s = (q . k) * scale              scale <= 0: 1/sqrt(head_dim)
+ *   s = softcap * tanh(s / softcap)  softcap > 0
+ *   s = s - slopes[head] * |i - j|   slopes not NULL ([n_heads] f32, device)
+ * and the keys a row sees are
+ *   (j <= i or j < prefix_lens[seq]) and j < ctx_lens[seq]
+ *   and (window <= 0 or i - j < window)
+ * with prefix_lens NULL: 0 ([batch] int32, device; prefill only).  A row that
+ * sees no key gives zeros. */
+typedef struct nyion_score_options {
+    float          scale;
+    float          softcap;
+    int32_t        window;
+    int32_t        reserved; /* 0 */
+    const float*   slopes;
+    const int32_t* prefix_lens;
+} nyion_score_options;
+
+/* Block tables and slots of a batch, from its lengths, on the device.
+ * Sequence b has cached_lens[b] tokens in the cache and gets new_lens[b] more
+ * (0: none; negative lengths count as 0).  Written:
+ *   ctx_lens[b]     cached_lens[b] + new_lens[b];
+ *   row_starts      [batch + 1], the running sum of new_lens: sequence b's new
+ *                   rows are row_starts[b] .. row_starts[b + 1] - 1;
+ *   block_tables    the entries of pages that begin behind cached_lens[b] and
+ *                   hold new tokens, taken from free_blocks in the order of
+ *                   (sequence, page); -1 once the list is used up.  Other
+ *                   entries are left as they are;
+ *   positions[r]    row r's position in its sequence (int32), and
+ *   slots[r]        block * block_tokens + position % block_tokens (int64),
+ *                   -1 where the row's page is past the table, or its block
+ *                   not in [0, num_blocks).  Rows of [row_starts[batch],
+ *                   n_rows), of a batch padded to n_rows, get -1 in both;
+ *   counts          [2]: the blocks wanted (those of pages inside the table;
+ *                   the first min(counts[0], n_free) of free_blocks are in
+ *                   use) and the rows, row_starts[batch].
+ * Rows past n_rows are not written.  No output may overlap an input.
+ * batch <= 4096, block_tokens a power of two; sums saturate at 2^31 - 1. */
+int nyion_batch_map(const int32_t* cached_lens, const int32_t* new_lens, int batch,
+                    const int32_t* free_blocks, int n_free, int block_tokens, int num_blocks,
+                    int32_t* block_tables, int max_blocks_per_seq, int32_t* ctx_lens,
+                    int32_t* row_starts, int64_t* slots, int32_t* positions, int n_rows,
+                    int32_t* counts, nyion_stream_t stream);
+
+/* Rows k, v [n_rows][n_kv_heads][head_dim] (io_dtype; consecutive rows
+ * k_stride and v_stride elements apart, as in a fused q/k/v projection) into
+ * the cache at slots[n_rows].  A row whose slot is not in [0, num_blocks *
+ * block_tokens) is skipped.
+ * Rows that go to one block lie one behind the other, with at most 62 skipped
+ * rows between two of them, as in what nyion_batch_map gives; a run is rows of
+ * one block with consecutive slots, and runs of one block are written in their
+ * order.  The tokens of the block in front of a run's first slot are live,
+ * those behind its last are not.  Per run and kv head, for K and V each:
+ *   scale = the smallest power of two (2^-126 at least) by which the run's
+ *           largest magnitude fits the codes (448 or 127), or the scale of the
+ *           live tokens if that is larger;
+ *   a live token's code becomes the nearest to its value under the new scale
+ *           (unchanged unless the scale grew), a new row's code the nearest to
+ *           x / scale, ties to even.
+ * With powers of two the division is exact and so is an e4m3 code's move to a
+ * larger scale, down to the format's subnormals: results depend on nothing
+ * but the values.  Integers give up at most one bit of their range for it.
+ * Infinities are stored as the largest code and NaN as 0, neither counts
+ * towards the scale, and nyion_take_status reports that there were some.
+ * Codes behind a run's last slot are left as they are.
+ * Rows are 16-byte aligned and so are the strides in bytes. */
+int nyion_kv8_write(const nyion_kv8_cache* cache, const int64_t* slots, int n_rows, const void* k,
+                    int64_t k_stride, const void* v, int64_t v_stride, int io_dtype,
+                    nyion_stream_t stream);
+
+/* Attention of one query row per sequence over the 8-bit cache: row b stands
+ * at position ctx_lens[b] - 1 and its own K/V are in the cache already.
+ * q, out [batch][n_heads][head_dim] of io_dtype, q_stride elements between
+ * rows of q (16-byte aligned rows), out contiguous and 16-byte aligned;
+ * q head h reads kv head h / (n_heads / n_kv_heads).
+ * block_tables [batch][max_blocks_per_seq]; tokens of entries that are not in
+ * [0, num_blocks), and tokens past the table, are skipped.  ctx_lens[b] <= 0:
+ * a padded entry, its row of out is zeros.  max_ctx, a bound of ctx_lens,
+ * shapes the launch and the workspace, not the result.  options NULL: none.
+ * q and the weights are carried as two binary16 terms each (22 bits) relative
+ * to the row's largest, sums in f32.  An infinity or NaN in a head of q makes
+ * that head's row of out NaN.
+ * d_workspace: nyion_kv8_decode_workspace_size bytes, 256-byte aligned,
+ * zero-filled before its first use (nyion_decode_workspace_init) and left with
+ * its counters at zero by every call; calls that may overlap in time, replays
+ * of captured graphs among them, need workspaces of their own. */
+size_t nyion_kv8_decode_workspace_size(const nyion_kv8_cache* cache, int batch, int n_heads,
+                                       int max_ctx, int window);
+int nyion_kv8_decode_attention(const nyion_kv8_cache* cache, const int32_t* block_tables,
+                               int max_blocks_per_seq, const int32_t* ctx_lens, int batch,
+                               int max_ctx, const void* q, int64_t q_stride, void* out, int n_heads,
+                               int io_dtype, const nyion_score_options* options,
+                               void* d_workspace, size_t workspace_bytes, nyion_stream_t stream);
 
 /* ------------------------------------------------------ Q4_K weight GEMV */
 

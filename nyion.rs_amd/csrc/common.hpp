@@ -60,7 +60,7 @@ int device_cu_count();
 // Range-status word of the current device: kernels OR a kRange* bit into it
 // when an input lies outside what a reduced-precision operand can hold;
 // nyion_take_status reads and clears it.  nullptr when there is no device.
-enum : unsigned { kRangePrefillV = 1u, kRangeDecodeQ = 2u };
+enum : unsigned { kRangePrefillV = 1u, kRangeDecodeQ = 2u, kRangeKv8Write = 4u };
 unsigned* device_status_word();
 
 // Records in the status word whether some of the n bf16 values of v reaches

@@ -1,0 +1,758 @@
+// kv8_decode.hip — batched decode attention over the 8-bit cache (gfx950).
+//
+// One query row per sequence.  A segment is one (sequence, kv head, group of
+// up to 16 q heads); its keys are cut into tiles of 64 positions, four
+// subtiles of 16, each inside one cache block and so with one K and one V
+// scale.  Per tile a wavefront computes, on v_mfma_f32_16x16x32_f16,
+//   S^T[16 tokens][16 heads] += K . Q^T     per subtile, K codes as binary16
+//   O^T[16 dims][16 heads]   += V^T . P^T   per 16 dims, over 32 tokens a time
+// Codes are exact in binary16; q and the weights p * (V scale) are two
+// binary16 terms each, which keeps 22 bits, so what is lost is below the f32
+// sums' own rounding.  Each takes two MFMAs for one, on a matrix unit that the
+// memory leaves idle for the most part.
+//
+// No operand passes through LDS or between lanes.  K arrives as 16 bytes per
+// lane in A's layout (row = token, 8 + 8 dims).  Row m of a subtile's A is
+// token 4 (m % 4) + m / 4, so the lane group g = lane / 16 of the result holds
+// tokens 4 i + g, i = 0..3: in V those are, for each i, four neighbouring rows,
+// which one load per i reads whole.  V^T's A operand needs one dim and eight
+// tokens per lane: the eight loads give a lane 4 (8 at head_dim 128) dims of
+// its eight tokens, and two byte permutes per pair of words put two tokens'
+// bytes side by side before the conversion that they need anyway.
+//
+// Scales: a subtile's K scale multiplies its scores (with the row's own power
+// of two, that of q, and 1/sqrt(D) log2(e)).  A V scale multiplies its weights
+// relative to the largest of the scales seen, times 2^14: every product is at
+// most 2^14 and keeps its 22 bits down to 2^-18 of the largest.
+//
+// Softmax in log2 units with a running maximum; O and the sum are rescaled
+// only in tiles that raise it.
+//
+// Split over keys: as many pieces as fill the chip, in one launch.  Batches
+// lay their segments' tiles end to end and cut the list into equal ranges, one
+// per workgroup, whatever the spread of the lengths; launches of few segments
+// cut each by itself, which needs no sums over the batch.  Pieces of a segment
+// leave their maximum, sum and O in the workspace (stored and loaded past the
+// L2s, which the XCDs do not share) and the last one to arrive joins them in
+// the order of the pieces, so that the order of arrival changes nothing.
+//
+// Bound: the cache's bytes at batch, the chain length -> table -> rows ->
+// partials -> join for single sequences.
+#include <limits.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "kv8.hpp"
+
+namespace nyion {
+
+constexpr int kTile = 64;            // tokens
+constexpr int kMaxSeqs = 1024;       // sequences per launch
+constexpr int kMaxWgs = 2048;        // workgroups per launch (sizes the workspace)
+constexpr int kWaves = 4;
+constexpr float kWeightUnit = 16384.f;
+constexpr float kLeastScale = 7.888609052210118e-31f;  // 2^-100
+
+struct Kv8DecodeArgs {
+    Kv8 c;
+    ScoreArgs s;
+    const int32_t* tables;
+    const int32_t* ctx_lens;
+    const void* q;
+    void* out;
+    long long q_stride;
+    float* ws_acc;   // [slots][16][D]
+    float2* ws_ml;   // [slots][16]
+    int* counters;   // [segments]
+    int max_blocks;
+    int span;        // tokens that a table covers
+    int batch;
+    int n_heads;
+    int group;       // q heads per kv head
+    int n_hg;        // head groups of 16 per kv head
+    int pieces;      // > 0: each segment is cut into up to this many pieces
+    int min_tiles;   // fewest tiles of a workgroup
+    int bf16;
+};
+
+// max(v, v of lane ^ 16), then ^ 32: the lanes of one head
+__device__ __forceinline__ float max_groups(float v) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float sum_groups(float v) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+__device__ __forceinline__ float lane_value(float v, int lane) {
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane));
+}
+
+// tanh: the odd series to x^11 below 0.35 (the next term is 2e-8 of x there),
+// 1 - 2 / (e^2x + 1) above, where that difference loses nothing.
+__device__ __forceinline__ float tanh_series(float x) {
+    const float y = x * x;
+    float t = -0.00886323553f;  // -1382/155925
+    t = __builtin_fmaf(t, y, 0.0218694885f);    // 62/2835
+    t = __builtin_fmaf(t, y, -0.0539682540f);   // -17/315
+    t = __builtin_fmaf(t, y, 0.133333333f);     // 2/15
+    t = __builtin_fmaf(t, y, -0.333333333f);
+    return __builtin_fmaf(t * y, x, x);
+}
+__device__ __forceinline__ float tanh_exp(float x) {
+    return 1.f - 2.f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * 2.885390081777927f) + 1.f);
+}
+
+template <int D>
+struct Kv8Tile {
+    static constexpr int KC = D / 64;  // 16-byte chunks of a K row per lane
+    static constexpr int VW = D / 64;  // words of a V row per lane
+    u32x4_t k[4][KC];
+    uint32_t v[4][4][VW];
+};
+
+// The range of keys of a sequence and its tiles.
+struct Kv8Span {
+    int lo, hi;      // keys [lo, hi)
+    int first;       // tile of lo
+    int tiles;       // at least 1: an empty range has a tile with every key masked
+};
+__device__ __forceinline__ Kv8Span kv8_span(const Kv8DecodeArgs& a, int b) {
+    Kv8Span r;
+    const int ctx = a.ctx_lens[b];
+    r.hi = max(min(ctx, a.span), 0);
+    r.lo = a.s.window > 0 && ctx > a.s.window ? ctx - a.s.window : 0;
+    if (r.lo > r.hi) r.lo = r.hi;
+    r.first = r.lo / kTile;
+    r.tiles = max((int)(((unsigned)r.hi + kTile - 1) / kTile) - r.first, 1);
+    return r;
+}
+
+template <int D, int CODE, bool MODS>
+__global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void kv8_decode_kernel(Kv8DecodeArgs a) {
+    using Tile = Kv8Tile<D>;
+    constexpr int KC = Tile::KC, VW = Tile::VW;
+    constexpr int MT = D / 16;       // 16-dim tiles of O^T
+    constexpr int PAD = 4;
+    __shared__ float sm_acc[kWaves][16][D + PAD];
+    __shared__ float2 sm_ml[kWaves][16];
+    __shared__ int sm_ends[kMaxSeqs];
+    __shared__ int sm_wave[kWaves];
+    __shared__ int sm_last;
+
+    const int tid = threadIdx.x;
+    const int lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n = lane & 15;   // head of the group / row of an A operand
+    const int g = lane >> 4;   // lane group
+    const int units = a.c.n_kv_heads * a.n_hg;
+
+    // where this workgroup's tiles lie
+    long long pos = 0, end = 0, total = 0;
+    long long wgs = 0;
+    if (a.pieces == 0) {
+        int before = 0;
+        for (int b0 = 0; b0 < a.batch; b0 += 64 * kWaves) {
+            const int b = b0 + tid;
+            int x = b < a.batch ? kv8_span(a, b).tiles : 0;
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) {
+                const int y = __shfl_up(x, d);
+                if (lane >= d) x += y;
+            }
+            if (lane == 63) sm_wave[wave] = x;
+            __syncthreads();
+            int all = 0;
+#pragma unroll
+            for (int w = 0; w < kWaves; w++) {
+                if (w < wave) x += sm_wave[w];
+                all += sm_wave[w];
+            }
+            if (b < a.batch) sm_ends[b] = before + x;
+            before += all;
+            __syncthreads();
+        }
+        total = (long long)__builtin_amdgcn_readfirstlane(before) * units;
+        wgs = min((long long)gridDim.x, (total + a.min_tiles - 1) / a.min_tiles);
+        if ((long long)blockIdx.x >= wgs) return;
+        pos = total * blockIdx.x / wgs;
+        end = total * (blockIdx.x + 1) / wgs;
+    }
+    bool first_segment = true;
+
+    while (true) {
+        int seg, t0, t1, n_pieces;
+        long long slot_mine, slot0, slot1;  // partials: piece 0's, and piece p >= 1's less stride (p - 1)
+        int slot_step;
+        Kv8Span sp;
+        int b;
+        if (a.pieces > 0) {
+            seg = (int)blockIdx.x / a.pieces;
+            const int p = (int)blockIdx.x - seg * a.pieces;
+            b = seg / units;
+            sp = kv8_span(a, b);
+            n_pieces = min(a.pieces, (sp.tiles + a.min_tiles - 1) / a.min_tiles);
+            if (p >= n_pieces) return;
+            t0 = (int)((long long)sp.tiles * p / n_pieces);
+            t1 = (int)((long long)sp.tiles * (p + 1) / n_pieces);
+            slot0 = (long long)seg * a.pieces;
+            slot1 = slot0 + 1;
+            slot_step = 1;
+            slot_mine = slot0 + p;
+        } else {
+            int lo = 0, hi = a.batch - 1;  // first sequence whose tiles end behind pos
+            while (lo < hi) {
+                const int mid = (lo + hi) >> 1;
+                if ((long long)sm_ends[mid] * units > pos)
+                    hi = mid;
+                else
+                    lo = mid + 1;
+            }
+            b = __builtin_amdgcn_readfirstlane(lo);
+            sp = kv8_span(a, b);
+            const long long seq0 = b > 0 ? (long long)sm_ends[b - 1] * units : 0;
+            const int unit = (int)((pos - seq0) / sp.tiles);
+            const long long start = seq0 + (long long)unit * sp.tiles;  // of the segment
+            seg = b * units + unit;
+            t0 = (int)(pos - start);
+            t1 = (int)min((long long)sp.tiles, end - start);
+            // workgroup w holds the tiles from total * w / wgs on
+            const long long w0 = ((start + 1) * wgs - 1) / total;
+            const long long w1 = ((start + sp.tiles) * wgs - 1) / total;
+            n_pieces = (int)(w1 - w0) + 1;
+            slot0 = 2 * w0 + (total * w0 / wgs >= start ? 0 : 1);
+            slot1 = 2 * (w0 + 1);
+            slot_step = 2;
+            slot_mine = 2 * (long long)blockIdx.x + (first_segment ? 0 : 1);
+        }
+        const int unit = seg - b * units;
+        const int kvh = unit / a.n_hg;
+        const int hg = unit - kvh * a.n_hg;
+        const int head0 = kvh * a.group + hg * 16;
+        const int heads = min(16, a.group - hg * 16);
+        const int32_t* table = a.tables + (long long)b * a.max_blocks;
+        const int qpos = a.ctx_lens[b] - 1;
+
+        // q of head n as two binary16 terms of q * 2^-e, largest in [2^13, 2^14)
+        half8_t qh[2 * KC], ql[2 * KC];
+        float crow;  // what a score is multiplied with, besides the K scale
+        {
+            float x[2 * KC][8];
+            float top = 0.f;
+            const bool on = n < heads;
+#pragma unroll
+            for (int c = 0; c < 2 * KC; c++) {
+                const long long at =
+                    b * a.q_stride + (long long)(head0 + n) * D + 64 * (c >> 1) + 16 * g + 8 * (c & 1);
+                if (!on) {
+#pragma unroll
+                    for (int e = 0; e < 8; e++) x[c][e] = 0.f;
+                } else if (a.bf16) {
+                    const u32x4_t w = *(const u32x4_t*)((const uint16_t*)a.q + at);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        x[c][2 * e] = __uint_as_float(w[e] << 16);
+                        x[c][2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+                    }
+                } else {
+                    const float4_t u = *(const float4_t*)((const float*)a.q + at);
+                    const float4_t v = *(const float4_t*)((const float*)a.q + at + 4);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) x[c][e] = u[e], x[c][4 + e] = v[e];
+                }
+#pragma unroll
+                for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[c][e]));
+            }
+            top = max_groups(top);
+            const int ex = top > 0.f && top <= 3.402823466e38f ? __builtin_amdgcn_frexp_expf(top) - 14 : 0;
+#pragma unroll
+            for (int c = 0; c < 2 * KC; c++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const float y = __builtin_amdgcn_ldexpf(x[c][e], -ex);
+                    const _Float16 hi = (_Float16)y;
+                    qh[c][e] = hi;
+                    ql[c][e] = (_Float16)(y - (float)hi);
+                }
+            crow = __builtin_amdgcn_ldexpf(a.s.scale_log2, ex);
+        }
+        float slope = 0.f;
+        if (MODS && a.s.slopes && n < heads) slope = a.s.slopes[head0 + n] * 1.4426950408889634f;
+
+        float4_t acc[MT];
+#pragma unroll
+        for (int j = 0; j < MT; j++) acc[j] = float4_t{};
+        float m = -INFINITY, l = 0.f;
+        float unit_scale = 0.f;  // largest V scale so far, what acc is measured in
+
+        // this wavefront's tiles
+        const int tn = t1 - t0;
+        int tw = sp.first + t0 + tn * wave / kWaves;
+        const int tw1 = sp.first + t0 + tn * (wave + 1) / kWaves;
+
+        const uint32_t klane = (uint32_t)((4 * (n & 3) + (n >> 2)) * D + 16 * g);
+        const uint32_t vlane = (uint32_t)(g * D + 4 * VW * n);
+
+        while (tw < tw1) {
+            // up to 16 tiles, 64 subtiles: a lane looks up one subtile's place and scales
+            const int nt = min(16, tw1 - tw);
+            const int tok = tw * kTile + 16 * lane;
+            int block = -1;
+            if (lane < 4 * nt && tok < sp.hi && tok + 16 > sp.lo) block = kv8_block(a.c, table, a.max_blocks, tok);
+            const bool present = block >= 0;
+            long long off = 0;
+            float ks = 0.f, vs = 0.f;
+            if (present) {
+                off = kv8_offset(a.c, block, kvh) + (long long)(tok & ((1 << a.c.bt_log2) - 1)) * D;
+                ks = a.c.k_scales[(long long)block * a.c.n_kv_heads + kvh];
+                vs = a.c.v_scales[(long long)block * a.c.n_kv_heads + kvh];
+            }
+            const unsigned long long absent = ~__ballot(present);
+            auto load = [&](Tile& t, int i) __attribute__((always_inline)) {
+#pragma unroll
+                for (int u = 0; u < 4; u++) {
+                    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)off, 4 * i + u);
+                    const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(off >> 32), 4 * i + u);
+                    const long long at = (long long)(((unsigned long long)hi << 32) | lo);
+                    const uint8_t* kb = a.c.k + at;
+                    const uint8_t* vb = a.c.v + at;
+#pragma unroll
+                    for (int c = 0; c < KC; c++) t.k[u][c] = *(const u32x4_t*)(kb + (klane + 64 * c));
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        if constexpr (VW == 2) {
+                            const u32x2_t w = *(const u32x2_t*)(vb + (vlane + 4 * D * r));
+                            t.v[u][r][0] = w[0];
+                            t.v[u][r][1] = w[1];
+                        } else {
+                            t.v[u][r][0] = *(const uint32_t*)(vb + (vlane + 4 * D * r));
+                        }
+                    }
+                }
+            };
+            Tile ta, tb;
+            load(ta, 0);
+            // the weights' unit: the largest V scale
+            {
+                const float top = fmaxf(wave_reduce_dpp<true>(fabsf(vs)), kLeastScale);
+                if (top > unit_scale) {
+                    const float down = unit_scale / top;
+#pragma unroll
+                    for (int j = 0; j < MT; j++) acc[j] *= down;
+                    unit_scale = top;
+                }
+            }
+            const float cvl = vs / unit_scale * kWeightUnit;
+
+            auto use = [&](Tile& t, int i) __attribute__((always_inline)) {
+                const int p0 = (tw + i) * kTile;
+                const int gone = (int)(absent >> (4 * i)) & 15;
+                const bool masked = p0 < sp.lo || p0 > sp.hi - kTile || gone;
+                float4_t s[4];
+#pragma unroll
+                for (int u = 0; u < 4; u++) {
+                    s[u] = float4_t{};
+#pragma unroll
+                    for (int c = 0; c < 2 * KC; c++) {
+                        const uint32_t w0 = kv8_bias<CODE>(t.k[u][c >> 1][2 * (c & 1)]);
+                        const uint32_t w1 = kv8_bias<CODE>(t.k[u][c >> 1][2 * (c & 1) + 1]);
+                        const u32x4_t kf = {kv8_pair<CODE, false>(w0), kv8_pair<CODE, true>(w0),
+                                            kv8_pair<CODE, false>(w1), kv8_pair<CODE, true>(w1)};
+                        const half8_t kh = __builtin_bit_cast(half8_t, kf);
+                        s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qh[c], s[u], 0, 0, 0);
+                        s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, ql[c], s[u], 0, 0, 0);
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < 4; u++) s[u] *= lane_value(ks, 4 * i + u) * crow;
+                if constexpr (MODS) {
+                    if (a.s.cap_log2 > 0.f) {
+                        float most = 0.f;
+#pragma unroll
+                        for (int u = 0; u < 4; u++)
+#pragma unroll
+                            for (int r = 0; r < 4; r++) most = fmaxf(most, fabsf(s[u][r]));
+                        const bool wide = __any(most > 0.35f);
+#pragma unroll
+                        for (int u = 0; u < 4; u++)
+#pragma unroll
+                            for (int r = 0; r < 4; r++) {
+                                float y = tanh_series(s[u][r]);
+                                if (wide) y = fabsf(s[u][r]) > 0.35f ? tanh_exp(s[u][r]) : y;
+                                s[u][r] = y * a.s.cap_log2;
+                            }
+                    }
+                    if (a.s.slopes) {
+                        const float back = (float)(qpos - p0 - g);
+#pragma unroll
+                        for (int u = 0; u < 4; u++)
+#pragma unroll
+                            for (int r = 0; r < 4; r++)
+                                s[u][r] = __builtin_fmaf(-slope, back - (float)(16 * u + 4 * r), s[u][r]);
+                    }
+                }
+                if (masked) {
+#pragma unroll
+                    for (int u = 0; u < 4; u++)
+#pragma unroll
+                        for (int r = 0; r < 4; r++) {
+                            const int key = p0 + 16 * u + 4 * r + g;
+                            const bool seen = key >= sp.lo && key < sp.hi && !((gone >> u) & 1);
+                            s[u][r] = seen ? s[u][r] : -INFINITY;
+#pragma unroll
+                            for (int x = 0; x < VW; x++) t.v[u][r][x] = seen ? t.v[u][r][x] : 0u;
+                        }
+                }
+                float top = -INFINITY;
+#pragma unroll
+                for (int u = 0; u < 4; u++)
+                    top = fmaxf(top, fmaxf(fmaxf(s[u][0], s[u][1]), fmaxf(s[u][2], s[u][3])));
+                top = fmaxf(m, max_groups(top));
+                const float base = top == -INFINITY ? 0.f : top;
+                if (__any(top > m)) {
+                    const float down = __builtin_amdgcn_exp2f(m - base);
+                    l *= down;
+#pragma unroll
+                    for (int j = 0; j < MT; j++) acc[j] *= down;
+                    m = top;
+                }
+                half8_t ph[2], pl[2];
+#pragma unroll
+                for (int u = 0; u < 4; u++) {
+                    const float cv = lane_value(cvl, 4 * i + u);
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const float p = __builtin_amdgcn_exp2f(s[u][r] - base);
+                        l += p;
+                        float w = p * cv;
+                        // one f32 value for both terms: the compiler may
+                        // otherwise round the product to binary16 by itself,
+                        // a unit away from the `hi` of the difference
+                        asm("" : "+v"(w));
+                        const _Float16 hi = (_Float16)w;
+                        ph[u >> 1][4 * (u & 1) + r] = hi;
+                        pl[u >> 1][4 * (u & 1) + r] = (_Float16)(w - (float)hi);
+                    }
+                }
+#pragma unroll
+                for (int pr = 0; pr < 2; pr++)
+#pragma unroll
+                    for (int x = 0; x < VW; x++) {
+                        uint32_t f[4][4];  // [dim within the word][token pair]
+#pragma unroll
+                        for (int tp = 0; tp < 4; tp++) {
+                            const uint32_t w0 = kv8_bias<CODE>(t.v[2 * pr + (tp >> 1)][2 * (tp & 1)][x]);
+                            const uint32_t w1 = kv8_bias<CODE>(t.v[2 * pr + (tp >> 1)][2 * (tp & 1) + 1][x]);
+                            const uint32_t lo = __builtin_amdgcn_perm(w1, w0, 0x05010400u);
+                            const uint32_t hi = __builtin_amdgcn_perm(w1, w0, 0x07030602u);
+                            f[0][tp] = kv8_pair<CODE, false>(lo);
+                            f[1][tp] = kv8_pair<CODE, true>(lo);
+                            f[2][tp] = kv8_pair<CODE, false>(hi);
+                            f[3][tp] = kv8_pair<CODE, true>(hi);
+                        }
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const half8_t vf =
+                                __builtin_bit_cast(half8_t, u32x4_t{f[e][0], f[e][1], f[e][2], f[e][3]});
+                            const int j = 4 * x + e;
+                            acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph[pr], acc[j], 0, 0, 0);
+                            acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl[pr], acc[j], 0, 0, 0);
+                        }
+                    }
+            };
+            int i = 0;
+            for (; i + 1 < nt; i += 2) {
+                load(tb, i + 1);
+                use(ta, i);
+                load(ta, min(i + 2, nt - 1));
+                use(tb, i + 1);
+            }
+            if (i < nt) use(ta, i);
+            tw += nt;
+        }
+
+        // the wavefronts' results through LDS
+        l = sum_groups(l);
+        {
+            const float back = unit_scale / kWeightUnit;
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+#pragma unroll
+                for (int x = 0; x < VW; x++)
+                    *(float4_t*)&sm_acc[wave][n][16 * VW * g + 4 * VW * r + 4 * x] =
+                        float4_t{acc[4 * x][r], acc[4 * x + 1][r], acc[4 * x + 2][r], acc[4 * x + 3][r]} * back;
+            if (g == 0) sm_ml[wave][n] = float2{m, l};
+        }
+        __syncthreads();
+        constexpr int DPT = D / 16;  // dims per thread
+        const int row = tid >> 4;
+        const int d0 = (tid & 15) * DPT;
+        float o[DPT];
+        float om = -INFINITY, ol = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWaves; w++) om = fmaxf(om, sm_ml[w][row].x);
+        const float obase = om == -INFINITY ? 0.f : om;
+#pragma unroll
+        for (int e = 0; e < DPT; e++) o[e] = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWaves; w++) {
+            const float2 ml = sm_ml[w][row];
+            const float f = __builtin_amdgcn_exp2f(ml.x - obase);
+            ol = __builtin_fmaf(ml.y, f, ol);
+#pragma unroll
+            for (int e = 0; e < DPT; e++) o[e] = __builtin_fmaf(sm_acc[w][row][d0 + e], f, o[e]);
+        }
+        auto write_out = [&]() {
+            if (row >= heads) return;
+            const float inv = ol == 0.f ? 0.f : 1.f / ol;  // nothing seen: zeros
+            const long long at = ((long long)b * a.n_heads + head0 + row) * D + d0;
+            if (a.bf16) {
+#pragma unroll
+                for (int e = 0; e < DPT; e += 4) {
+                    typedef __bf16 bf16x4_t __attribute__((ext_vector_type(4)));
+                    *(bf16x4_t*)((uint16_t*)a.out + at + e) =
+                        bf16x4_t{(__bf16)(o[e] * inv), (__bf16)(o[e + 1] * inv), (__bf16)(o[e + 2] * inv),
+                                 (__bf16)(o[e + 3] * inv)};
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < DPT; e += 4)
+                    *(float4_t*)((float*)a.out + at + e) =
+                        float4_t{o[e] * inv, o[e + 1] * inv, o[e + 2] * inv, o[e + 3] * inv};
+            }
+        };
+        if (n_pieces == 1) {
+            write_out();
+        } else {
+            if (row < heads) {
+                const __amdgpu_buffer_rsrc_t racc = partial_rsrc(a.ws_acc + slot_mine * 16 * D, 16 * D * 4);
+                const __amdgpu_buffer_rsrc_t rml = partial_rsrc(a.ws_ml + slot_mine * 16, 16 * 8);
+#pragma unroll
+                for (int e = 0; e < DPT; e += 4)
+                    __builtin_amdgcn_raw_buffer_store_b128(
+                        u32x4_t{__float_as_uint(o[e]), __float_as_uint(o[e + 1]), __float_as_uint(o[e + 2]),
+                                __float_as_uint(o[e + 3])},
+                        racc, (row * D + d0 + e) * 4, 0, kSc1);
+                if ((tid & 15) == 0)
+                    __builtin_amdgcn_raw_buffer_store_b64(u32x2_t{__float_as_uint(om), __float_as_uint(ol)}, rml,
+                                                          row * 8, 0, kSc1);
+            }
+            // every wavefront's stores have completed before the arrival is counted
+            __atomic_signal_fence(__ATOMIC_SEQ_CST);
+            __builtin_amdgcn_s_waitcnt(0);
+            __syncthreads();
+            if (tid == 0)
+                sm_last = __hip_atomic_fetch_add(a.counters + seg, 1, __ATOMIC_RELAXED,
+                                                 __HIP_MEMORY_SCOPE_AGENT) == n_pieces - 1;
+            __syncthreads();
+            if (sm_last) {
+                om = -INFINITY;
+                ol = 0.f;
+#pragma unroll
+                for (int e = 0; e < DPT; e++) o[e] = 0.f;
+                constexpr int AHEAD = 8;
+                for (int p = 0; p < n_pieces; p += AHEAD) {
+                    u32x4_t w[AHEAD][DPT / 4];
+                    u32x2_t ml[AHEAD];
+#pragma unroll
+                    for (int k = 0; k < AHEAD; k++) {
+                        const int pk = min(p + k, n_pieces - 1);
+                        const long long slot = pk == 0 ? slot0 : slot1 + (long long)slot_step * (pk - 1);
+                        const __amdgpu_buffer_rsrc_t racc = partial_rsrc(a.ws_acc + slot * 16 * D, 16 * D * 4);
+                        const __amdgpu_buffer_rsrc_t rml = partial_rsrc(a.ws_ml + slot * 16, 16 * 8);
+                        const int rr = min(row, heads - 1);  // rows behind the last hold nothing
+                        ml[k] = __builtin_amdgcn_raw_buffer_load_b64(rml, rr * 8, 0, kSc1);
+#pragma unroll
+                        for (int e = 0; e < DPT / 4; e++)
+                            w[k][e] = __builtin_amdgcn_raw_buffer_load_b128(racc, (rr * D + d0 + 4 * e) * 4, 0, kSc1);
+                    }
+                    float top = om;
+#pragma unroll
+                    for (int k = 0; k < AHEAD; k++) top = fmaxf(top, __uint_as_float(ml[k][0]));
+                    const float base = top == -INFINITY ? 0.f : top;
+                    const float down = __builtin_amdgcn_exp2f(om - base);
+                    om = top;
+                    ol *= down;
+#pragma unroll
+                    for (int e = 0; e < DPT; e++) o[e] *= down;
+#pragma unroll
+                    for (int k = 0; k < AHEAD; k++) {
+                        if (p + k >= n_pieces) break;
+                        const float f = __builtin_amdgcn_exp2f(__uint_as_float(ml[k][0]) - base);
+                        ol = __builtin_fmaf(__uint_as_float(ml[k][1]), f, ol);
+#pragma unroll
+                        for (int e = 0; e < DPT; e++)
+                            o[e] = __builtin_fmaf(__uint_as_float(w[k][e >> 2][e & 3]), f, o[e]);
+                    }
+                }
+                write_out();
+                if (tid == 0) __hip_atomic_store(a.counters + seg, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+        }
+        if (a.pieces > 0) return;
+        pos += t1 - t0;
+        first_segment = false;
+        if (pos >= end) return;
+        __syncthreads();  // LDS is free for the next segment
+    }
+}
+
+// ------------------------------------------------------------- host side
+
+// Tiles per workgroup at least, one per wavefront; a launch of at most
+// kDirectSegments segments cuts each of them by itself.
+constexpr int kMinTiles = 4;
+constexpr int kDirectSegments = 64;
+
+struct Kv8DecodePlan {
+    int units, chunk, pieces, grid;
+    size_t acc, ml, bytes;
+};
+
+static int decode_plan(Kv8DecodePlan& p, const Kv8& c, int batch, int n_heads, int max_ctx, int window,
+                       const char* what) {
+    if (batch <= 0 || n_heads <= 0 || max_ctx <= 0)
+        return set_error(NYION_ERR_INVALID, "%s: batch, n_heads and max_ctx must be positive", what);
+    if (n_heads % c.n_kv_heads)
+        return set_error(NYION_ERR_INVALID, "%s: n_heads %d not a multiple of n_kv_heads %d", what, n_heads,
+                         c.n_kv_heads);
+    if (n_heads > 16384) return set_error(NYION_ERR_UNSUPPORTED, "%s: n_heads %d", what, n_heads);
+    const int group = n_heads / c.n_kv_heads;
+    p.units = c.n_kv_heads * ((group + 15) / 16);
+    p.chunk = std::min(batch, kMaxSeqs);
+    const long long segments = (long long)p.chunk * p.units;
+    const long long keys = window > 0 ? std::min((long long)window + kTile, (long long)max_ctx) : max_ctx;
+    const long long tiles = (keys + kTile - 1) / kTile;
+    if (segments <= kDirectSegments) {
+        const long long fill = std::max(2 * device_cu_count() / segments, 1LL);
+        p.pieces = (int)std::min(fill, (tiles + kMinTiles - 1) / kMinTiles);
+        p.grid = (int)(segments * p.pieces);
+    } else {
+        p.pieces = 0;
+        p.grid = (int)std::min((long long)kMaxWgs, (tiles * segments + kMinTiles - 1) / kMinTiles);
+    }
+    const size_t slots = p.pieces ? (size_t)p.grid : 2 * (size_t)p.grid;
+    p.acc = slots * 16 * c.head_dim * sizeof(float);
+    p.ml = (slots * 16 * sizeof(float2) + 255) & ~(size_t)255;
+    p.bytes = p.acc + p.ml + (((size_t)segments * sizeof(int) + 255) & ~(size_t)255);
+    if (p.pieces == 1) p.bytes = 0;
+    return NYION_OK;
+}
+
+template <int D, int CODE, bool MODS>
+static int resident_wgs() {
+    static std::atomic<int> cache[kMaxDevices];
+    return per_device_value(
+        cache,
+        [] {
+            int per_cu = 0;
+            if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, kv8_decode_kernel<D, CODE, MODS>, 64 * kWaves,
+                                                             0) != hipSuccess) {
+                (void)hipGetLastError();
+                return 0;
+            }
+            return std::max(per_cu, 1) * device_cu_count();
+        },
+        512);
+}
+
+template <int D, int CODE, bool MODS>
+static void launch_decode(const Kv8DecodeArgs& a, int grid, hipStream_t stream) {
+    if (a.pieces == 0) grid = std::min(grid, resident_wgs<D, CODE, MODS>());
+    hipLaunchKernelGGL((kv8_decode_kernel<D, CODE, MODS>), dim3(grid), dim3(64 * kWaves), 0, stream, a);
+}
+
+}  // namespace nyion
+
+using namespace nyion;
+
+extern "C" {
+
+size_t nyion_kv8_decode_workspace_size(const nyion_kv8_cache* cache, int batch, int n_heads,
+                                       int max_ctx, int window) {
+    clear_error();
+    Kv8 c;
+    Kv8DecodePlan p;
+    if (kv8_cache_args(c, cache, "kv8_decode_workspace_size") != NYION_OK ||
+        decode_plan(p, c, batch, n_heads, max_ctx, window, "kv8_decode_workspace_size") != NYION_OK)
+        return 0;
+    return p.bytes;
+}
+
+int nyion_kv8_decode_attention(const nyion_kv8_cache* cache, const int32_t* block_tables,
+                               int max_blocks_per_seq, const int32_t* ctx_lens, int batch,
+                               int max_ctx, const void* q, int64_t q_stride, void* out, int n_heads,
+                               int io_dtype, const nyion_score_options* options,
+                               void* d_workspace, size_t workspace_bytes, nyion_stream_t stream) {
+    clear_error();
+    int rc;
+    if ((rc = require_device()) != NYION_OK) return rc;
+    const char* what = "kv8_decode";
+    Kv8DecodeArgs a;
+    Kv8DecodePlan p;
+    if ((rc = kv8_cache_args(a.c, cache, what)) != NYION_OK) return rc;
+    if ((rc = kv8_score_args(a.s, options, a.c.head_dim, false, what)) != NYION_OK) return rc;
+    if ((rc = decode_plan(p, a.c, batch, n_heads, max_ctx, a.s.window, what)) != NYION_OK) return rc;
+    if (io_dtype != NYION_IO_F32 && io_dtype != NYION_IO_BF16)
+        return set_error(NYION_ERR_INVALID, "%s: io_dtype %d", what, io_dtype);
+    if (!block_tables || !ctx_lens || !q || !out || max_blocks_per_seq <= 0)
+        return set_error(NYION_ERR_INVALID, "%s: null pointer, or max_blocks_per_seq not positive", what);
+    const int64_t size = io_dtype == NYION_IO_F32 ? 4 : 2, row = (int64_t)n_heads * a.c.head_dim;
+    if (q_stride < row)
+        return set_error(NYION_ERR_INVALID, "%s: q_stride %lld below n_heads * head_dim", what, (long long)q_stride);
+    if (!aligned(q, 16) || !aligned(out, 16) || q_stride * size % 16)
+        return set_error(NYION_ERR_INVALID, "%s: rows of q and out must be 16-byte aligned", what);
+    if (p.bytes) {
+        if (!d_workspace || workspace_bytes < p.bytes)
+            return set_error(NYION_ERR_WORKSPACE, "%s: workspace %zu bytes < required %zu", what,
+                             d_workspace ? workspace_bytes : (size_t)0, p.bytes);
+        if (!aligned(d_workspace, 256))
+            return set_error(NYION_ERR_INVALID, "%s: workspace not 256-byte aligned", what);
+    }
+    a.ws_acc = (float*)d_workspace;
+    a.ws_ml = (float2*)((char*)d_workspace + p.acc);
+    a.counters = (int*)((char*)d_workspace + p.acc + p.ml);
+    a.q_stride = q_stride;
+    a.max_blocks = max_blocks_per_seq;
+    a.span = (int)std::min((long long)max_blocks_per_seq << a.c.bt_log2, (long long)INT_MAX - 2 * kTile);
+    a.n_heads = n_heads;
+    a.group = n_heads / a.c.n_kv_heads;
+    a.n_hg = (a.group + 15) / 16;
+    a.pieces = p.pieces;
+    a.min_tiles = kMinTiles;
+    a.bf16 = io_dtype == NYION_IO_BF16;
+    const bool mods = a.s.cap_log2 > 0.f || a.s.slopes;
+    for (int b0 = 0; b0 < batch; b0 += p.chunk) {
+        a.batch = std::min(p.chunk, batch - b0);
+        a.tables = block_tables + (int64_t)b0 * max_blocks_per_seq;
+        a.ctx_lens = ctx_lens + b0;
+        a.q = (const char*)q + b0 * q_stride * size;
+        a.out = (char*)out + b0 * row * size;
+        auto by_mods = [&](auto d, auto code) {
+            constexpr int D = decltype(d)::value, CODE = decltype(code)::value;
+            if (mods)
+                launch_decode<D, CODE, true>(a, p.grid, (hipStream_t)stream);
+            else
+                launch_decode<D, CODE, false>(a, p.grid, (hipStream_t)stream);
+        };
+        auto by_code = [&](auto d) {
+            if (cache->code == NYION_KV8_E4M3)
+                by_mods(d, std::integral_constant<int, NYION_KV8_E4M3>{});
+            else
+                by_mods(d, std::integral_constant<int, NYION_KV8_INT8>{});
+        };
+        if (a.c.head_dim == 64)
+            by_code(std::integral_constant<int, 64>{});
+        else
+            by_code(std::integral_constant<int, 128>{});
+        if ((rc = check_launch(what)) != NYION_OK) return rc;
+    }
+    return NYION_OK;
+}
+
+}  // extern "C"

@@ -212,6 +212,8 @@ int nyion_take_status(nyion_stream_t stream) {
     if (got & kRangeDecodeQ)
         msg += "binary16 / Q4-20B KV decode: a q value of magnitude >= 65520 overflows the binary16 high "
                "part of q; the heads holding it are not valid. ";
+    if (got & kRangeKv8Write)
+        msg += "8-bit KV write: a K or V value was infinite (stored as the largest code) or NaN (stored as 0). ";
     return set_error(NYION_ERR_RANGE, "%s", msg.c_str());
 }
 

@@ -19,6 +19,12 @@ KV_F32 = 0
 KV_Q4_20B = 1
 KV_F16 = 2
 
+KV8_E4M3 = 0
+KV8_INT8 = 1
+
+IO_F32 = 0
+IO_BF16 = 1
+
 MEM_HOST_PINNED = 0
 MEM_DEVICE_LOCAL = 1
 MEM_UNIFIED_MAPPED = 2
@@ -61,6 +67,18 @@ class FuguConfig(C.Structure):
 class AttentionStrategy(C.Structure):
     _fields_ = [("kind", C.c_int32), ("window", C.c_int32), ("num_random", C.c_int32),
                 ("sentinel_stride", C.c_int32), ("num_dspark", C.c_int32), ("_pad", C.c_int32)]
+
+
+class Kv8CacheStruct(C.Structure):
+    _fields_ = [("k_codes", C.c_void_p), ("v_codes", C.c_void_p), ("k_scales", C.c_void_p),
+                ("v_scales", C.c_void_p), ("num_blocks", C.c_int32), ("n_kv_heads", C.c_int32),
+                ("block_tokens", C.c_int32), ("head_dim", C.c_int32), ("code", C.c_int32),
+                ("reserved", C.c_int32)]
+
+
+class ScoreOptionsStruct(C.Structure):
+    _fields_ = [("scale", C.c_float), ("softcap", C.c_float), ("window", C.c_int32),
+                ("reserved", C.c_int32), ("slopes", C.c_void_p), ("prefix_lens", C.c_void_p)]
 
 
 ATTN_FULL, ATTN_SPARSE, ATTN_SPARSE_DSPARK = 0, 1, 2
@@ -146,6 +164,12 @@ SIGNATURES = {
     "nyion_kv_pool_stats": (i32, [vp, C.POINTER(C.c_int64), C.POINTER(C.c_int64),
                                   C.POINTER(C.c_int64), C.POINTER(C.c_int64)]),
     "nyion_kv_pool_cold_slot": (vp, [vp, i32]),
+    "nyion_batch_map": (i32, [vp, vp, i32, vp, i32, i32, i32, vp, i32, vp, vp, vp, vp, i32, vp,
+                              vp]),
+    "nyion_kv8_write": (i32, [vp, vp, i32, vp, i64, vp, i64, i32, vp]),
+    "nyion_kv8_decode_workspace_size": (sz, [vp, i32, i32, i32, i32]),
+    "nyion_kv8_decode_attention": (i32, [vp, vp, i32, vp, i32, i32, vp, i64, vp, i32, i32, vp, vp,
+                                         sz, vp]),
     "nyion_gemv_q4k": (i32, [vp, vp, vp, i32, i32, vp]),
     "nyion_gemv_q4k_multi": (i32, [vp, vp, vp, vp, i32, i32, vp]),
     "nyion_gemv_q4k_batched": (i32, [vp, vp, i64, vp, i64, i32, i32, i32, vp]),
@@ -582,6 +606,178 @@ def kv_gather(pool, block_table, block_tokens, n_kv_heads, head_dim, kv_dtype, n
                                 n_kv_heads, head_dim, kv_dtype, n_tokens, ptr(out),
                                 stream_handle(stream))
     check(rc, "nyion_kv_gather")
+
+
+# ----------------------------------------------------------------------------
+# batched serving on an 8-bit cache
+# ----------------------------------------------------------------------------
+
+def _want(ok, what: str) -> None:
+    if not ok:
+        raise NyionError(ERR_INVALID, what)
+
+
+def _on_current_device(*tensors) -> bool:
+    torch = _torch()
+    dev = torch.cuda.current_device()
+    return all(t is None or (t.is_cuda and t.get_device() == dev) for t in tensors)
+
+
+def _io_dtype(t) -> int:
+    torch = _torch()
+    if t.dtype == torch.float32:
+        return IO_F32
+    _want(t.dtype == torch.bfloat16, f"rows are float32 or bfloat16, not {t.dtype}")
+    return IO_BF16
+
+
+def _check_rows(t, heads, head_dim, what) -> None:
+    """[rows][heads][head_dim], rows any distance apart."""
+    _want(t.dim() == 3 and t.shape[1] == heads and t.shape[2] == head_dim,
+          f"{what} is [rows][{heads}][{head_dim}], not {tuple(t.shape)}")
+    s = t.stride()
+    _want(s[2] == 1 and (s[1] == head_dim or heads == 1), f"{what}: a row is contiguous")
+
+
+def _check_int(t, torch_dtype, what, n=None) -> None:
+    _want(t.dtype == torch_dtype and t.is_contiguous(), f"{what} is contiguous {torch_dtype}")
+    _want(n is None or t.numel() == n, f"{what} has {n} entries, not {t.numel()}")
+
+
+class Kv8Cache:
+    """The handle of an 8-bit cache: k, v uint8 [num_blocks][Hkv][block_tokens][D] codes (the
+    bits of e4m3 or int8 values), k_scales, v_scales f32 [num_blocks][Hkv].  Keeps the tensors."""
+
+    def __init__(self, k, v, k_scales, v_scales, code=KV8_E4M3):
+        torch = _torch()
+        _want(k.dim() == 4 and v.shape == k.shape and k.element_size() == 1
+              and v.element_size() == 1, "k and v are one-byte [blocks][kv heads][tokens][dim]")
+        _want(k_scales.shape == k.shape[:2] and v_scales.shape == k.shape[:2]
+              and k_scales.dtype == v_scales.dtype == torch.float32,
+              "scales are float32 [blocks][kv heads]")
+        tensors = (k, v, k_scales, v_scales)
+        _want(all(t.is_contiguous() for t in tensors), "the cache's tensors are contiguous")
+        _want(len({t.device for t in tensors}) == 1, "the cache's tensors are on one device")
+        self.k, self.v, self.k_scales, self.v_scales, self.code = *tensors, code
+        self.num_blocks, self.n_kv_heads, self.block_tokens, self.head_dim = k.shape
+        self.device_index = k.get_device()
+        self.struct = Kv8CacheStruct(ptr(k), ptr(v), ptr(k_scales), ptr(v_scales), *k.shape, code, 0)
+        self.ref = C.addressof(self.struct)
+
+    @classmethod
+    def empty(cls, num_blocks, n_kv_heads, block_tokens, head_dim, code=KV8_E4M3, device="cuda"):
+        """A cache without live rows."""
+        torch = _torch()
+        shape = (num_blocks, n_kv_heads, block_tokens, head_dim)
+        k, v = (torch.zeros(shape, dtype=torch.uint8, device=device) for _ in range(2))
+        ks, vs = (torch.zeros(shape[:2], dtype=torch.float32, device=device) for _ in range(2))
+        return cls(k, v, ks, vs, code)
+
+    def check_device(self) -> None:
+        _want(self.device_index == _torch().cuda.current_device(),
+              "the cache is on another device than the current one")
+
+
+class ScoreOptions:
+    """What happens to a score before the softmax: scale (0: 1/sqrt(D)), softcap, window, slopes
+    [n_heads] f32 (bias by distance), prefix_lens [B] int32 (prefill).  Keeps the tensors."""
+
+    def __init__(self, scale=0.0, softcap=0.0, window=0, slopes=None, prefix_lens=None):
+        torch = _torch()
+        if slopes is not None:
+            _want(slopes.dtype == torch.float32 and slopes.is_contiguous(),
+                  "slopes are contiguous float32")
+        if prefix_lens is not None:
+            _check_int(prefix_lens, torch.int32, "prefix_lens")
+        self.slopes, self.prefix_lens, self.window = slopes, prefix_lens, window
+        self.struct = ScoreOptionsStruct(scale, softcap, window, 0, ptr(slopes), ptr(prefix_lens))
+        self.ref = C.addressof(self.struct)
+
+    def check(self, n_heads, batch) -> None:
+        _want(self.slopes is None or self.slopes.numel() == n_heads,
+              f"slopes have {n_heads} entries")
+        _want(self.prefix_lens is None or self.prefix_lens.numel() == batch,
+              f"prefix_lens have {batch} entries")
+        _want(_on_current_device(self.slopes, self.prefix_lens),
+              "the options' tensors are on the current device")
+
+
+def batch_map(cached_lens, new_lens, free_blocks, block_tables, block_tokens, num_blocks, ctx_lens,
+              row_starts, slots, positions, counts, stream=None):
+    """Slots, positions and new pages of a batch: cached_lens, new_lens [B], free_blocks [n] and
+    block_tables [B][max_blocks] (updated) int32; written: ctx_lens [B], row_starts [B + 1],
+    positions [n_rows], counts [2] int32 and slots [n_rows] int64."""
+    torch = _torch()
+    B = cached_lens.numel()
+    for t, what, n in ((cached_lens, "cached_lens", B), (new_lens, "new_lens", B),
+                       (free_blocks, "free_blocks", None), (ctx_lens, "ctx_lens", B),
+                       (block_tables, "block_tables", None), (row_starts, "row_starts", B + 1),
+                       (positions, "positions", slots.numel()), (counts, "counts", 2)):
+        _check_int(t, torch.int32, what, n)
+    _check_int(slots, torch.int64, "slots")
+    _want(block_tables.dim() == 2 and block_tables.shape[0] == B, f"block_tables is [{B}][blocks]")
+    _want(_on_current_device(cached_lens, new_lens, free_blocks, block_tables, ctx_lens, row_starts,
+                             slots, positions, counts), "tensors are on the current device")
+    rc = load().nyion_batch_map(
+        ptr(cached_lens), ptr(new_lens), B, ptr(free_blocks), free_blocks.numel(), block_tokens,
+        num_blocks, ptr(block_tables), block_tables.shape[1], ptr(ctx_lens), ptr(row_starts),
+        ptr(slots), ptr(positions), slots.numel(), ptr(counts), stream_handle(stream))
+    check(rc, "nyion_batch_map")
+
+
+def kv8_write(cache, slots, k, v, stream=None):
+    """Rows k, v [n_rows][Hkv][D] (f32 or bf16, rows any distance apart) into the cache at
+    slots [n_rows] int64, as batch_map gives them."""
+    torch = _torch()
+    cache.check_device()
+    for t, what in ((k, "k"), (v, "v")):
+        _check_rows(t, cache.n_kv_heads, cache.head_dim, what)
+    _want(k.dtype == v.dtype and k.shape == v.shape, "k and v are alike")
+    _check_int(slots, torch.int64, "slots", k.shape[0])
+    _want(_on_current_device(slots, k, v), "tensors are on the current device")
+    rc = load().nyion_kv8_write(cache.ref, ptr(slots), k.shape[0], ptr(k), k.stride(0), ptr(v),
+                                v.stride(0), _io_dtype(k), stream_handle(stream))
+    check(rc, "nyion_kv8_write")
+
+
+def kv8_decode_workspace_size(cache, batch, n_heads, max_ctx, window=0) -> int:
+    return int(load().nyion_kv8_decode_workspace_size(cache.ref, batch, n_heads, max_ctx, window))
+
+
+def _check_attention(cache, q, block_tables, ctx_lens, out, options):
+    torch = _torch()
+    cache.check_device()
+    n_heads, B = q.shape[1], ctx_lens.numel()
+    _check_rows(q, n_heads, cache.head_dim, "q")
+    _want(out.shape == q.shape and out.dtype == q.dtype and out.is_contiguous(),
+          "out is contiguous and has q's shape and type")
+    _check_int(ctx_lens, torch.int32, "ctx_lens")
+    _check_int(block_tables, torch.int32, "block_tables")
+    _want(block_tables.dim() == 2 and block_tables.shape[0] == B, f"block_tables is [{B}][blocks]")
+    _want(_on_current_device(q, block_tables, ctx_lens, out), "tensors are on the current device")
+    if options is not None:
+        options.check(n_heads, B)
+    return n_heads, B
+
+
+def kv8_decode(cache, q, block_tables, ctx_lens, out, max_ctx=None, options=None, workspace=None,
+               stream=None):
+    """Attention of one row per sequence over the cache: q, out [B][Hq][D] f32 or bf16,
+    block_tables [B][max_blocks], ctx_lens [B] int32.  Returns the workspace."""
+    n_heads, B = _check_attention(cache, q, block_tables, ctx_lens, out, options)
+    _want(q.shape[0] == B, f"q has {B} rows")
+    if max_ctx is None:
+        max_ctx = max(int(ctx_lens.max().item()), 1)
+    if workspace is None:
+        workspace = alloc_workspace(kv8_decode_workspace_size(
+            cache, B, n_heads, max_ctx, 0 if options is None else options.window), q.device)
+    ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
+    rc = load().nyion_kv8_decode_attention(
+        cache.ref, ptr(block_tables), block_tables.shape[1], ptr(ctx_lens), B, max_ctx, ptr(q),
+        q.stride(0), ptr(out), n_heads, _io_dtype(q), None if options is None else options.ref,
+        ptr(workspace), ws_bytes, stream_handle(stream))
+    check(rc, "nyion_kv8_decode_attention")
+    return workspace
 
 
 # Reference-shaped zone pools (PagedKVCache geometry): pools are 1-D device
