@@ -579,9 +579,10 @@ int nyion_q4_quantize(const float* in, int64_t n_rows, int head_dim, uint8_t* ou
 /* No counterpart in the reference, which serves one sequence at a time from
  * f32 and Q4-20B pages (swamp-engine/src/cache.rs).  A step of a batch is
  * three calls, none of which needs the host to know a length exactly:
- *   nyion_batch_map             lengths -> slots, positions, new pages;
- *   nyion_kv8_write             each layer's new K/V rows -> the 8-bit cache;
- *   nyion_kv8_decode_attention  one query row per sequence.
+ *   nyion_batch_map       lengths -> slots, positions, new pages;
+ *   nyion_kv8_write       each layer's new K/V rows -> the 8-bit cache;
+ *   nyion_kv8_decode_attention, one query row per sequence, or
+ *   nyion_kv8_prefill_attention_bf16, any number of rows per sequence.
  *
  * The cache holds K and V codes [num_blocks][n_kv_heads][block_tokens]
  * [head_dim], one byte each, and one f32 scale per (block, kv head) for each
@@ -704,6 +705,27 @@ int nyion_kv8_decode_attention(const nyion_kv8_cache* cache, const int32_t* bloc
                                int max_ctx, const void* q, int64_t q_stride, void* out, int n_heads,
                                int io_dtype, const nyion_score_options* options,
                                void* d_workspace, size_t workspace_bytes, nyion_stream_t stream);
+
+/* Attention of a ragged batch over the 8-bit cache, bf16 q and out: rows
+ * row_starts[b] .. row_starts[b + 1] - 1 (row_starts [batch + 1] int32, rising,
+ * from 0) of q [n_rows][n_heads][head_dim] are the last tokens of sequence b,
+ * row r at position ctx_lens[b] - row_starts[b + 1] + r; their K/V are in the
+ * cache already.  Rows behind row_starts[batch] are left as they are in out,
+ * and rows at negative positions give zeros.  max_rows and max_ctx, bounds of
+ * the rows and the length of one sequence, shape the launch and the
+ * workspace, not the result.  q is carried exactly (bf16 relative to the
+ * row's largest value in binary16), weights and V in binary16 (11 bits), sums
+ * in f32; n_rows * n_heads at most 2^27.  Everything else as for
+ * nyion_kv8_decode_attention. */
+size_t nyion_kv8_prefill_workspace_size(const nyion_kv8_cache* cache, int batch, int n_heads,
+                                        int n_rows, int max_rows, int max_ctx, int window);
+int nyion_kv8_prefill_attention_bf16(const nyion_kv8_cache* cache, const int32_t* block_tables,
+                                     int max_blocks_per_seq, const int32_t* ctx_lens,
+                                     const int32_t* row_starts, int batch, int n_rows,
+                                     int max_rows, int max_ctx, const uint16_t* q,
+                                     int64_t q_stride, uint16_t* out, int n_heads,
+                                     const nyion_score_options* options, void* d_workspace,
+                                     size_t workspace_bytes, nyion_stream_t stream);
 
 /* ------------------------------------------------------ Q4_K weight GEMV */
 

@@ -430,7 +430,7 @@ int kv8_score_args(ScoreArgs& s, const nyion_score_options* o, int head_dim, boo
     const double log2e = 1.4426950408889634;
     s.scale_log2 = (float)(o->softcap > 0.f ? scale / o->softcap : scale * log2e);
     s.cap_log2 = (float)(o->softcap * log2e);
-    s.window = o->window > 0 ? o->window : 0;
+    s.window = o->window > 0 ? std::min(o->window, 1 << 30) : 0;  // sums with a position stay in 32 bits
     s.slopes = o->slopes;
     s.prefix_lens = o->prefix_lens;
     return NYION_OK;

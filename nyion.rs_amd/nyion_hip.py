@@ -170,6 +170,9 @@ SIGNATURES = {
     "nyion_kv8_decode_workspace_size": (sz, [vp, i32, i32, i32, i32]),
     "nyion_kv8_decode_attention": (i32, [vp, vp, i32, vp, i32, i32, vp, i64, vp, i32, i32, vp, vp,
                                          sz, vp]),
+    "nyion_kv8_prefill_workspace_size": (sz, [vp, i32, i32, i32, i32, i32, i32]),
+    "nyion_kv8_prefill_attention_bf16": (i32, [vp, vp, i32, vp, vp, i32, i32, i32, i32, vp, i64,
+                                               vp, i32, vp, vp, sz, vp]),
     "nyion_gemv_q4k": (i32, [vp, vp, vp, i32, i32, vp]),
     "nyion_gemv_q4k_multi": (i32, [vp, vp, vp, vp, i32, i32, vp]),
     "nyion_gemv_q4k_batched": (i32, [vp, vp, i64, vp, i64, i32, i32, i32, vp]),
@@ -777,6 +780,38 @@ def kv8_decode(cache, q, block_tables, ctx_lens, out, max_ctx=None, options=None
         q.stride(0), ptr(out), n_heads, _io_dtype(q), None if options is None else options.ref,
         ptr(workspace), ws_bytes, stream_handle(stream))
     check(rc, "nyion_kv8_decode_attention")
+    return workspace
+
+
+def kv8_prefill_workspace_size(cache, batch, n_heads, n_rows, max_rows, max_ctx, window=0) -> int:
+    return int(load().nyion_kv8_prefill_workspace_size(cache.ref, batch, n_heads, n_rows, max_rows,
+                                                       max_ctx, window))
+
+
+def kv8_prefill_bf16(cache, q, block_tables, ctx_lens, row_starts, out, max_rows=None, max_ctx=None,
+                     options=None, workspace=None, stream=None):
+    """Attention of a ragged batch over the cache: q, out [n_rows][Hq][D] bf16, the rows of sequence
+    b, row_starts [B + 1] int32, being its last tokens.  Returns the workspace."""
+    torch = _torch()
+    n_heads, B = _check_attention(cache, q, block_tables, ctx_lens, out, options)
+    _want(q.dtype == torch.bfloat16, f"q is bfloat16, not {q.dtype}")
+    _check_int(row_starts, torch.int32, "row_starts", B + 1)
+    _want(_on_current_device(row_starts), "row_starts is on the current device")
+    n_rows = q.shape[0]
+    if max_rows is None:
+        max_rows = max(int((row_starts[1:] - row_starts[:-1]).max().item()), 1)
+    if max_ctx is None:
+        max_ctx = max(int(ctx_lens.max().item()), 1)
+    if workspace is None:
+        workspace = alloc_workspace(kv8_prefill_workspace_size(
+            cache, B, n_heads, n_rows, max_rows, max_ctx, 0 if options is None else options.window),
+            q.device)
+    ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
+    rc = load().nyion_kv8_prefill_attention_bf16(
+        cache.ref, ptr(block_tables), block_tables.shape[1], ptr(ctx_lens), ptr(row_starts), B,
+        n_rows, max_rows, max_ctx, ptr(q), q.stride(0), ptr(out), n_heads,
+        None if options is None else options.ref, ptr(workspace), ws_bytes, stream_handle(stream))
+    check(rc, "nyion_kv8_prefill_attention_bf16")
     return workspace
 
 
