@@ -73,6 +73,7 @@ struct Kv8DecodeArgs {
     int n_hg;        // head groups of 16 per kv head
     int pieces;      // > 0: each segment is cut into up to this many pieces
     int min_tiles;   // fewest tiles of a workgroup
+    int slots;       // partials that the workspace holds
     int bf16;
 };
 
@@ -91,6 +92,17 @@ __device__ __forceinline__ float sum_groups(float v) {
 }
 __device__ __forceinline__ float lane_value(float v, int lane) {
     return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane));
+}
+
+// What two f32 values have beyond their binary16 parts, as binary16: exact
+// differences, each one mixed-precision FMA instead of a conversion and a
+// subtraction.
+__device__ __forceinline__ half2_t rest_of_pair(half2_t hi, float a, float b) {
+    const uint32_t h = __builtin_bit_cast(uint32_t, hi);
+    float x, y;
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(x) : "v"(h), "v"(a));
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(y) : "v"(h), "v"(b));
+    return half2_t{(_Float16)x, (_Float16)y};
 }
 
 // tanh: the odd series to x^11 below 0.35 (the next term is 2e-8 of x there),
@@ -152,38 +164,58 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void kv8_decode_kerne
     const int g = lane >> 4;   // lane group
     const int units = a.c.n_kv_heads * a.n_hg;
 
-    // where this workgroup's tiles lie
-    long long pos = 0, end = 0, total = 0;
-    long long wgs = 0;
+    // Where this workgroup's tiles lie: of `total` tiles each of `wgs`
+    // workgroups takes total / wgs, the first total % wgs one more.
+    uint32_t pos = 0, end = 0, wgs = 0, share = 0, extra = 0;
+    int seq_end = 0;  // up to 64 sequences: lane b holds the tiles up to and with b
     if (a.pieces == 0) {
-        int before = 0;
-        for (int b0 = 0; b0 < a.batch; b0 += 64 * kWaves) {
-            const int b = b0 + tid;
-            int x = b < a.batch ? kv8_span(a, b).tiles : 0;
+        uint32_t total;
+        if (a.batch <= 64) {
+            seq_end = lane < a.batch ? kv8_span(a, lane).tiles : 0;
 #pragma unroll
             for (int d = 1; d < 64; d <<= 1) {
-                const int y = __shfl_up(x, d);
-                if (lane >= d) x += y;
+                const int y = __shfl_up(seq_end, d);
+                if (lane >= d) seq_end += y;
             }
-            if (lane == 63) sm_wave[wave] = x;
-            __syncthreads();
-            int all = 0;
+            total = (uint32_t)__builtin_amdgcn_readlane(seq_end, 63) * units;
+        } else {
+            int before = 0;
+            for (int b0 = 0; b0 < a.batch; b0 += 64 * kWaves) {
+                const int b = b0 + tid;
+                int x = b < a.batch ? kv8_span(a, b).tiles : 0;
 #pragma unroll
-            for (int w = 0; w < kWaves; w++) {
-                if (w < wave) x += sm_wave[w];
-                all += sm_wave[w];
+                for (int d = 1; d < 64; d <<= 1) {
+                    const int y = __shfl_up(x, d);
+                    if (lane >= d) x += y;
+                }
+                if (lane == 63) sm_wave[wave] = x;
+                __syncthreads();
+                int all = 0;
+#pragma unroll
+                for (int w = 0; w < kWaves; w++) {
+                    if (w < wave) x += sm_wave[w];
+                    all += sm_wave[w];
+                }
+                if (b < a.batch) sm_ends[b] = before + x;
+                before += all;
+                __syncthreads();
             }
-            if (b < a.batch) sm_ends[b] = before + x;
-            before += all;
-            __syncthreads();
+            total = (uint32_t)__builtin_amdgcn_readfirstlane(before) * units;
         }
-        total = (long long)__builtin_amdgcn_readfirstlane(before) * units;
-        wgs = min((long long)gridDim.x, (total + a.min_tiles - 1) / a.min_tiles);
-        if ((long long)blockIdx.x >= wgs) return;
-        pos = total * blockIdx.x / wgs;
-        end = total * (blockIdx.x + 1) / wgs;
+        wgs = min((uint32_t)gridDim.x, (total + a.min_tiles - 1) / a.min_tiles);
+        if (blockIdx.x >= wgs) return;
+        share = total / wgs;
+        extra = total - share * wgs;
+        pos = share * blockIdx.x + min(blockIdx.x, extra);
+        end = pos + share + (blockIdx.x < extra ? 1 : 0);
     }
     bool first_segment = true;
+    // the workgroup that holds tile t, and the first tile of workgroup w
+    const auto holder = [&](uint32_t t) {
+        const uint32_t longer = extra * (share + 1);
+        return t < longer ? t / (share + 1) : extra + (t - longer) / share;
+    };
+    const auto first_tile = [&](uint32_t w) { return share * w + min(w, extra); };
 
     while (true) {
         int seg, t0, t1, n_pieces;
@@ -198,37 +230,49 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void kv8_decode_kerne
             sp = kv8_span(a, b);
             n_pieces = min(a.pieces, (sp.tiles + a.min_tiles - 1) / a.min_tiles);
             if (p >= n_pieces) return;
-            t0 = (int)((long long)sp.tiles * p / n_pieces);
-            t1 = (int)((long long)sp.tiles * (p + 1) / n_pieces);
+            // pieces of tiles / n_pieces, the first ones one more
+            const int part = sp.tiles / n_pieces, more = sp.tiles - part * n_pieces;
+            t0 = part * p + min(p, more);
+            t1 = t0 + part + (p < more ? 1 : 0);
             slot0 = (long long)seg * a.pieces;
             slot1 = slot0 + 1;
             slot_step = 1;
             slot_mine = slot0 + p;
         } else {
-            int lo = 0, hi = a.batch - 1;  // first sequence whose tiles end behind pos
-            while (lo < hi) {
-                const int mid = (lo + hi) >> 1;
-                if ((long long)sm_ends[mid] * units > pos)
-                    hi = mid;
-                else
-                    lo = mid + 1;
+            int before;  // tiles of the sequences in front
+            if (a.batch <= 64) {
+                b = (int)__builtin_ctzll(__ballot((uint32_t)seq_end * units > pos));
+                before = b > 0 ? __builtin_amdgcn_readlane(seq_end, b - 1) : 0;
+            } else {
+                int lo = 0, hi = a.batch - 1;  // first sequence whose tiles end behind pos
+                while (lo < hi) {
+                    const int mid = (lo + hi) >> 1;
+                    if ((uint32_t)sm_ends[mid] * units > pos)
+                        hi = mid;
+                    else
+                        lo = mid + 1;
+                }
+                b = __builtin_amdgcn_readfirstlane(lo);
+                before = b > 0 ? __builtin_amdgcn_readfirstlane(sm_ends[b - 1]) : 0;
             }
-            b = __builtin_amdgcn_readfirstlane(lo);
             sp = kv8_span(a, b);
-            const long long seq0 = b > 0 ? (long long)sm_ends[b - 1] * units : 0;
-            const int unit = (int)((pos - seq0) / sp.tiles);
-            const long long start = seq0 + (long long)unit * sp.tiles;  // of the segment
-            seg = b * units + unit;
+            const uint32_t seq0 = (uint32_t)before * units;
+            const uint32_t unit = (pos - seq0) / (uint32_t)sp.tiles;
+            const uint32_t start = seq0 + unit * sp.tiles;  // of the segment
+            seg = b * units + (int)unit;
             t0 = (int)(pos - start);
-            t1 = (int)min((long long)sp.tiles, end - start);
-            // workgroup w holds the tiles from total * w / wgs on
-            const long long w0 = ((start + 1) * wgs - 1) / total;
-            const long long w1 = ((start + sp.tiles) * wgs - 1) / total;
-            n_pieces = (int)(w1 - w0) + 1;
-            slot0 = 2 * w0 + (total * w0 / wgs >= start ? 0 : 1);
-            slot1 = 2 * (w0 + 1);
+            t1 = (int)min((uint32_t)sp.tiles, end - start);
+            if (t0 == 0 && t1 == sp.tiles) {
+                n_pieces = 1;
+                slot0 = slot1 = slot_mine = 0;
+            } else {
+                const uint32_t w0 = holder(start), w1 = holder(start + sp.tiles - 1);
+                n_pieces = (int)(w1 - w0) + 1;
+                slot0 = 2 * (long long)w0 + (first_tile(w0) >= start ? 0 : 1);
+                slot1 = 2 * (long long)(w0 + 1);
+                slot_mine = 2 * (long long)blockIdx.x + (first_segment ? 0 : 1);
+            }
             slot_step = 2;
-            slot_mine = 2 * (long long)blockIdx.x + (first_segment ? 0 : 1);
         }
         const int unit = seg - b * units;
         const int kvh = unit / a.n_hg;
@@ -238,49 +282,6 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void kv8_decode_kerne
         const int32_t* table = a.tables + (long long)b * a.max_blocks;
         const int qpos = a.ctx_lens[b] - 1;
 
-        // q of head n as two binary16 terms of q * 2^-e, largest in [2^13, 2^14)
-        half8_t qh[2 * KC], ql[2 * KC];
-        float crow;  // what a score is multiplied with, besides the K scale
-        {
-            float x[2 * KC][8];
-            float top = 0.f;
-            const bool on = n < heads;
-#pragma unroll
-            for (int c = 0; c < 2 * KC; c++) {
-                const long long at =
-                    b * a.q_stride + (long long)(head0 + n) * D + 64 * (c >> 1) + 16 * g + 8 * (c & 1);
-                if (!on) {
-#pragma unroll
-                    for (int e = 0; e < 8; e++) x[c][e] = 0.f;
-                } else if (a.bf16) {
-                    const u32x4_t w = *(const u32x4_t*)((const uint16_t*)a.q + at);
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        x[c][2 * e] = __uint_as_float(w[e] << 16);
-                        x[c][2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
-                    }
-                } else {
-                    const float4_t u = *(const float4_t*)((const float*)a.q + at);
-                    const float4_t v = *(const float4_t*)((const float*)a.q + at + 4);
-#pragma unroll
-                    for (int e = 0; e < 4; e++) x[c][e] = u[e], x[c][4 + e] = v[e];
-                }
-#pragma unroll
-                for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[c][e]));
-            }
-            top = max_groups(top);
-            const int ex = top > 0.f && top <= 3.402823466e38f ? __builtin_amdgcn_frexp_expf(top) - 14 : 0;
-#pragma unroll
-            for (int c = 0; c < 2 * KC; c++)
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const float y = __builtin_amdgcn_ldexpf(x[c][e], -ex);
-                    const _Float16 hi = (_Float16)y;
-                    qh[c][e] = hi;
-                    ql[c][e] = (_Float16)(y - (float)hi);
-                }
-            crow = __builtin_amdgcn_ldexpf(a.s.scale_log2, ex);
-        }
         float slope = 0.f;
         if (MODS && a.s.slopes && n < heads) slope = a.s.slopes[head0 + n] * 1.4426950408889634f;
 
@@ -298,45 +299,98 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void kv8_decode_kerne
         const uint32_t klane = (uint32_t)((4 * (n & 3) + (n >> 2)) * D + 16 * g);
         const uint32_t vlane = (uint32_t)(g * D + 4 * VW * n);
 
-        while (tw < tw1) {
-            // up to 16 tiles, 64 subtiles: a lane looks up one subtile's place and scales
-            const int nt = min(16, tw1 - tw);
-            const int tok = tw * kTile + 16 * lane;
+        // up to 16 tiles, 64 subtiles, from tile t on: a lane looks up one
+        // subtile's place and scales
+        long long off = 0;
+        float ks = 0.f, vs = 0.f;
+        unsigned long long absent = 0;
+        auto look_up = [&](int t) __attribute__((always_inline)) {
+            const int tok = t * kTile + 16 * lane;
             int block = -1;
-            if (lane < 4 * nt && tok < sp.hi && tok + 16 > sp.lo) block = kv8_block(a.c, table, a.max_blocks, tok);
+            if (lane < 4 * (tw1 - t) && tok < sp.hi && tok + 16 > sp.lo) block = kv8_block(a.c, table, a.max_blocks, tok);
             const bool present = block >= 0;
-            long long off = 0;
-            float ks = 0.f, vs = 0.f;
+            off = 0;
+            ks = vs = 0.f;
             if (present) {
                 off = kv8_offset(a.c, block, kvh) + (long long)(tok & ((1 << a.c.bt_log2) - 1)) * D;
                 ks = a.c.k_scales[(long long)block * a.c.n_kv_heads + kvh];
                 vs = a.c.v_scales[(long long)block * a.c.n_kv_heads + kvh];
             }
-            const unsigned long long absent = ~__ballot(present);
-            auto load = [&](Tile& t, int i) __attribute__((always_inline)) {
+            absent = ~__ballot(present);
+        };
+        auto load = [&](Tile& t, int i) __attribute__((always_inline)) {
 #pragma unroll
-                for (int u = 0; u < 4; u++) {
-                    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)off, 4 * i + u);
-                    const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(off >> 32), 4 * i + u);
-                    const long long at = (long long)(((unsigned long long)hi << 32) | lo);
-                    const uint8_t* kb = a.c.k + at;
-                    const uint8_t* vb = a.c.v + at;
+            for (int u = 0; u < 4; u++) {
+                const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)off, 4 * i + u);
+                const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(off >> 32), 4 * i + u);
+                const long long at = (long long)(((unsigned long long)hi << 32) | lo);
+                const uint8_t* kb = a.c.k + at;
+                const uint8_t* vb = a.c.v + at;
 #pragma unroll
-                    for (int c = 0; c < KC; c++) t.k[u][c] = *(const u32x4_t*)(kb + (klane + 64 * c));
+                for (int c = 0; c < KC; c++) t.k[u][c] = *(const u32x4_t*)(kb + (klane + 64 * c));
 #pragma unroll
-                    for (int r = 0; r < 4; r++) {
-                        if constexpr (VW == 2) {
-                            const u32x2_t w = *(const u32x2_t*)(vb + (vlane + 4 * D * r));
-                            t.v[u][r][0] = w[0];
-                            t.v[u][r][1] = w[1];
-                        } else {
-                            t.v[u][r][0] = *(const uint32_t*)(vb + (vlane + 4 * D * r));
-                        }
+                for (int r = 0; r < 4; r++) {
+                    if constexpr (VW == 2) {
+                        const u32x2_t w = *(const u32x2_t*)(vb + (vlane + 4 * D * r));
+                        t.v[u][r][0] = w[0];
+                        t.v[u][r][1] = w[1];
+                    } else {
+                        t.v[u][r][0] = *(const uint32_t*)(vb + (vlane + 4 * D * r));
                     }
                 }
-            };
-            Tile ta, tb;
-            load(ta, 0);
+            }
+        };
+        // the first tile's rows are on their way while q is split
+        Tile ta, tb;
+        if (tw < tw1) look_up(tw);
+        // q of head n as two binary16 terms of q * 2^-e, largest in [2^13, 2^14)
+        half8_t qh[2 * KC], ql[2 * KC];
+        float crow;  // what a score is multiplied with, besides the K scale
+        float xq[2 * KC][8];
+#pragma unroll
+        for (int c = 0; c < 2 * KC; c++) {
+            const long long at = b * a.q_stride + (long long)(head0 + n) * D + 64 * (c >> 1) + 16 * g + 8 * (c & 1);
+            if (n >= heads) {
+#pragma unroll
+                for (int e = 0; e < 8; e++) xq[c][e] = 0.f;
+            } else if (a.bf16) {
+                const u32x4_t w = *(const u32x4_t*)((const uint16_t*)a.q + at);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    xq[c][2 * e] = __uint_as_float(w[e] << 16);
+                    xq[c][2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+                }
+            } else {
+                const float4_t u = *(const float4_t*)((const float*)a.q + at);
+                const float4_t v = *(const float4_t*)((const float*)a.q + at + 4);
+#pragma unroll
+                for (int e = 0; e < 4; e++) xq[c][e] = u[e], xq[c][4 + e] = v[e];
+            }
+        }
+        if (tw < tw1) load(ta, 0);
+        {
+            float top = 0.f;
+#pragma unroll
+            for (int c = 0; c < 2 * KC; c++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(xq[c][e]));
+            top = max_groups(top);
+            const int ex = top > 0.f && top <= 3.402823466e38f ? __builtin_amdgcn_frexp_expf(top) - 14 : 0;
+#pragma unroll
+            for (int c = 0; c < 2 * KC; c++)
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) {
+                    const float y0 = __builtin_amdgcn_ldexpf(xq[c][e], -ex), y1 = __builtin_amdgcn_ldexpf(xq[c][e + 1], -ex);
+                    const half2_t hi = {(_Float16)y0, (_Float16)y1};
+                    const half2_t lo = rest_of_pair(hi, y0, y1);
+                    qh[c][e] = hi[0], qh[c][e + 1] = hi[1];
+                    ql[c][e] = lo[0], ql[c][e + 1] = lo[1];
+                }
+            crow = __builtin_amdgcn_ldexpf(a.s.scale_log2, ex);
+        }
+
+        while (tw < tw1) {
+            const int nt = min(16, tw1 - tw);
             // the weights' unit: the largest V scale
             {
                 const float top = fmaxf(wave_reduce_dpp<true>(fabsf(vs)), kLeastScale);
@@ -353,24 +407,36 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void kv8_decode_kerne
                 const int p0 = (tw + i) * kTile;
                 const int gone = (int)(absent >> (4 * i)) & 15;
                 const bool masked = p0 < sp.lo || p0 > sp.hi - kTile || gone;
+                // the four subtiles' chains side by side: a chain's MFMAs wait for each other
                 float4_t s[4];
 #pragma unroll
-                for (int u = 0; u < 4; u++) {
-                    s[u] = float4_t{};
+                for (int u = 0; u < 4; u++) s[u] = float4_t{};
 #pragma unroll
-                    for (int c = 0; c < 2 * KC; c++) {
+                for (int c = 0; c < 2 * KC; c++) {
+                    half8_t kh[4];
+#pragma unroll
+                    for (int u = 0; u < 4; u++) {
                         const uint32_t w0 = kv8_bias<CODE>(t.k[u][c >> 1][2 * (c & 1)]);
                         const uint32_t w1 = kv8_bias<CODE>(t.k[u][c >> 1][2 * (c & 1) + 1]);
                         const u32x4_t kf = {kv8_pair<CODE, false>(w0), kv8_pair<CODE, true>(w0),
                                             kv8_pair<CODE, false>(w1), kv8_pair<CODE, true>(w1)};
-                        const half8_t kh = __builtin_bit_cast(half8_t, kf);
-                        s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qh[c], s[u], 0, 0, 0);
-                        s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, ql[c], s[u], 0, 0, 0);
+                        kh[u] = __builtin_bit_cast(half8_t, kf);
+                        s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh[u], qh[c], s[u], 0, 0, 0);
                     }
-                }
 #pragma unroll
-                for (int u = 0; u < 4; u++) s[u] *= lane_value(ks, 4 * i + u) * crow;
+                    for (int u = 0; u < 4; u++)
+                        s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh[u], ql[c], s[u], 0, 0, 0);
+                }
+                // log2 scores are s * f
+                float f[4];
+#pragma unroll
+                for (int u = 0; u < 4; u++) f[u] = lane_value(ks, 4 * i + u) * crow;
                 if constexpr (MODS) {
+#pragma unroll
+                    for (int u = 0; u < 4; u++) {
+                        s[u] *= f[u];
+                        f[u] = 1.f;
+                    }
                     if (a.s.cap_log2 > 0.f) {
                         float most = 0.f;
 #pragma unroll
@@ -397,21 +463,24 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void kv8_decode_kerne
                     }
                 }
                 if (masked) {
+                    asm volatile("");  // a branch: 80 instructions that few tiles need
 #pragma unroll
-                    for (int u = 0; u < 4; u++)
+                    for (int u = 0; u < 4; u++) {
 #pragma unroll
                         for (int r = 0; r < 4; r++) {
                             const int key = p0 + 16 * u + 4 * r + g;
                             const bool seen = key >= sp.lo && key < sp.hi && !((gone >> u) & 1);
-                            s[u][r] = seen ? s[u][r] : -INFINITY;
+                            s[u][r] = seen ? s[u][r] * f[u] : -INFINITY;
 #pragma unroll
                             for (int x = 0; x < VW; x++) t.v[u][r][x] = seen ? t.v[u][r][x] : 0u;
                         }
+                        f[u] = 1.f;
+                    }
                 }
                 float top = -INFINITY;
 #pragma unroll
                 for (int u = 0; u < 4; u++)
-                    top = fmaxf(top, fmaxf(fmaxf(s[u][0], s[u][1]), fmaxf(s[u][2], s[u][3])));
+                    top = fmaxf(top, fmaxf(fmaxf(s[u][0], s[u][1]), fmaxf(s[u][2], s[u][3])) * f[u]);
                 top = fmaxf(m, max_groups(top));
                 const float base = top == -INFINITY ? 0.f : top;
                 if (__any(top > m)) {
@@ -425,18 +494,25 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void kv8_decode_kerne
 #pragma unroll
                 for (int u = 0; u < 4; u++) {
                     const float cv = lane_value(cvl, 4 * i + u);
+                    float w[4];
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
-                        const float p = __builtin_amdgcn_exp2f(s[u][r] - base);
+                        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][r], f[u], -base));
                         l += p;
-                        float w = p * cv;
-                        // one f32 value for both terms: the compiler may
-                        // otherwise round the product to binary16 by itself,
-                        // a unit away from the `hi` of the difference
-                        asm("" : "+v"(w));
-                        const _Float16 hi = (_Float16)w;
-                        ph[u >> 1][4 * (u & 1) + r] = hi;
-                        pl[u >> 1][4 * (u & 1) + r] = (_Float16)(w - (float)hi);
+                        w[r] = p * cv;
+                        // one f32 value for both terms: the compiler may otherwise
+                        // round the product to binary16 by itself, a unit away from
+                        // the part that the rest is taken from
+                        asm("" : "+v"(w[r]));
+                    }
+#pragma unroll
+                    for (int r = 0; r < 4; r += 2) {
+                        const half2_t hi = {(_Float16)w[r], (_Float16)w[r + 1]};
+                        const half2_t lo = rest_of_pair(hi, w[r], w[r + 1]);
+                        ph[u >> 1][4 * (u & 1) + r] = hi[0];
+                        ph[u >> 1][4 * (u & 1) + r + 1] = hi[1];
+                        pl[u >> 1][4 * (u & 1) + r] = lo[0];
+                        pl[u >> 1][4 * (u & 1) + r + 1] = lo[1];
                     }
                 }
 #pragma unroll
@@ -474,6 +550,10 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void kv8_decode_kerne
             }
             if (i < nt) use(ta, i);
             tw += nt;
+            if (tw < tw1) {
+                look_up(tw);
+                load(ta, 0);
+            }
         }
 
         // the wavefronts' results through LDS
@@ -529,18 +609,19 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void kv8_decode_kerne
         if (n_pieces == 1) {
             write_out();
         } else {
+            const __amdgpu_buffer_rsrc_t racc = partial_rsrc(a.ws_acc, (uint32_t)a.slots * 16 * D * 4);
+            const __amdgpu_buffer_rsrc_t rml = partial_rsrc(a.ws_ml, (uint32_t)a.slots * 16 * 8);
             if (row < heads) {
-                const __amdgpu_buffer_rsrc_t racc = partial_rsrc(a.ws_acc + slot_mine * 16 * D, 16 * D * 4);
-                const __amdgpu_buffer_rsrc_t rml = partial_rsrc(a.ws_ml + slot_mine * 16, 16 * 8);
+                const int mine = (int)slot_mine * 16 + row;
 #pragma unroll
                 for (int e = 0; e < DPT; e += 4)
                     __builtin_amdgcn_raw_buffer_store_b128(
                         u32x4_t{__float_as_uint(o[e]), __float_as_uint(o[e + 1]), __float_as_uint(o[e + 2]),
                                 __float_as_uint(o[e + 3])},
-                        racc, (row * D + d0 + e) * 4, 0, kSc1);
+                        racc, (mine * D + d0 + e) * 4, 0, kSc1);
                 if ((tid & 15) == 0)
                     __builtin_amdgcn_raw_buffer_store_b64(u32x2_t{__float_as_uint(om), __float_as_uint(ol)}, rml,
-                                                          row * 8, 0, kSc1);
+                                                          mine * 8, 0, kSc1);
             }
             // every wavefront's stores have completed before the arrival is counted
             __atomic_signal_fence(__ATOMIC_SEQ_CST);
@@ -551,25 +632,30 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void kv8_decode_kerne
                                                  __HIP_MEMORY_SCOPE_AGENT) == n_pieces - 1;
             __syncthreads();
             if (sm_last) {
+                // 16 threads a head; what is left of the workgroup takes every
+                // `groups`-th piece, so that one round of loads has many
+                const int rows = heads > 8 ? 16 : heads > 4 ? 8 : heads > 2 ? 4 : heads;  // a power of two
+                const int groups = 16 / rows;
+                const int mrow = row & (rows - 1), mgrp = row / rows;
+                const int rr = min(mrow, heads - 1);  // rows behind the last hold nothing
                 om = -INFINITY;
                 ol = 0.f;
 #pragma unroll
                 for (int e = 0; e < DPT; e++) o[e] = 0.f;
                 constexpr int AHEAD = 8;
-                for (int p = 0; p < n_pieces; p += AHEAD) {
+                for (int p = mgrp; p < n_pieces; p += AHEAD * groups) {
                     u32x4_t w[AHEAD][DPT / 4];
                     u32x2_t ml[AHEAD];
 #pragma unroll
                     for (int k = 0; k < AHEAD; k++) {
-                        const int pk = min(p + k, n_pieces - 1);
-                        const long long slot = pk == 0 ? slot0 : slot1 + (long long)slot_step * (pk - 1);
-                        const __amdgpu_buffer_rsrc_t racc = partial_rsrc(a.ws_acc + slot * 16 * D, 16 * D * 4);
-                        const __amdgpu_buffer_rsrc_t rml = partial_rsrc(a.ws_ml + slot * 16, 16 * 8);
-                        const int rr = min(row, heads - 1);  // rows behind the last hold nothing
-                        ml[k] = __builtin_amdgcn_raw_buffer_load_b64(rml, rr * 8, 0, kSc1);
+                        const int pk = min(p + k * groups, n_pieces - 1);
+                        const int slot = (int)(pk == 0 ? slot0 : slot1 + slot_step * (pk - 1));
+                        // slots are at most 2 * kMaxWgs: their bytes stay in 32 bits
+                        ml[k] = __builtin_amdgcn_raw_buffer_load_b64(rml, (slot * 16 + rr) * 8, 0, kSc1);
 #pragma unroll
                         for (int e = 0; e < DPT / 4; e++)
-                            w[k][e] = __builtin_amdgcn_raw_buffer_load_b128(racc, (rr * D + d0 + 4 * e) * 4, 0, kSc1);
+                            w[k][e] = __builtin_amdgcn_raw_buffer_load_b128(
+                                racc, ((slot * 16 + rr) * D + d0 + 4 * e) * 4, 0, kSc1);
                     }
                     float top = om;
 #pragma unroll
@@ -582,12 +668,35 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void kv8_decode_kerne
                     for (int e = 0; e < DPT; e++) o[e] *= down;
 #pragma unroll
                     for (int k = 0; k < AHEAD; k++) {
-                        if (p + k >= n_pieces) break;
+                        if (p + k * groups >= n_pieces) break;
                         const float f = __builtin_amdgcn_exp2f(__uint_as_float(ml[k][0]) - base);
                         ol = __builtin_fmaf(__uint_as_float(ml[k][1]), f, ol);
 #pragma unroll
                         for (int e = 0; e < DPT; e++)
                             o[e] = __builtin_fmaf(__uint_as_float(w[k][e >> 2][e & 3]), f, o[e]);
+                    }
+                }
+                if (groups > 1) {
+                    float* const part = &sm_acc[0][0][0];  // [groups * rows = 16][D + PAD]
+#pragma unroll
+                    for (int e = 0; e < DPT; e++) part[row * (D + PAD) + d0 + e] = o[e];
+                    if ((tid & 15) == 0) sm_ml[0][row] = float2{om, ol};
+                    __syncthreads();
+                    om = -INFINITY;
+                    ol = 0.f;
+#pragma unroll
+                    for (int e = 0; e < DPT; e++) o[e] = 0.f;
+                    if (row < rows) {
+                        for (int k = 0; k < groups; k++) om = fmaxf(om, sm_ml[0][k * rows + row].x);
+                        const float base = om == -INFINITY ? 0.f : om;
+                        for (int k = 0; k < groups; k++) {
+                            const float2 ml = sm_ml[0][k * rows + row];
+                            const float f = __builtin_amdgcn_exp2f(ml.x - base);
+                            ol = __builtin_fmaf(ml.y, f, ol);
+#pragma unroll
+                            for (int e = 0; e < DPT; e++)
+                                o[e] = __builtin_fmaf(part[(k * rows + row) * (D + PAD) + d0 + e], f, o[e]);
+                        }
                     }
                 }
                 write_out();
@@ -611,6 +720,7 @@ constexpr int kDirectSegments = 64;
 
 struct Kv8DecodePlan {
     int units, chunk, pieces, grid;
+    int slots;
     size_t acc, ml, bytes;
 };
 
@@ -636,7 +746,8 @@ static int decode_plan(Kv8DecodePlan& p, const Kv8& c, int batch, int n_heads, i
         p.pieces = 0;
         p.grid = (int)std::min((long long)kMaxWgs, (tiles * segments + kMinTiles - 1) / kMinTiles);
     }
-    const size_t slots = p.pieces ? (size_t)p.grid : 2 * (size_t)p.grid;
+    p.slots = p.pieces ? p.grid : 2 * p.grid;
+    const size_t slots = (size_t)p.slots;
     p.acc = slots * 16 * c.head_dim * sizeof(float);
     p.ml = (slots * 16 * sizeof(float2) + 255) & ~(size_t)255;
     p.bytes = p.acc + p.ml + (((size_t)segments * sizeof(int) + 255) & ~(size_t)255);
@@ -725,10 +836,17 @@ int nyion_kv8_decode_attention(const nyion_kv8_cache* cache, const int32_t* bloc
     a.n_hg = (a.group + 15) / 16;
     a.pieces = p.pieces;
     a.min_tiles = kMinTiles;
+    a.slots = p.slots;
     a.bf16 = io_dtype == NYION_IO_BF16;
     const bool mods = a.s.cap_log2 > 0.f || a.s.slopes;
-    for (int b0 = 0; b0 < batch; b0 += p.chunk) {
-        a.batch = std::min(p.chunk, batch - b0);
+    int chunk = p.chunk;
+    if (!p.pieces) {  // a launch numbers its tiles in 32 bits
+        const long long per_seq = (long long)p.units * (a.span / kTile + 2);
+        chunk = (int)std::min((long long)chunk, (long long)INT_MAX / per_seq);
+        if (chunk < 1) return set_error(NYION_ERR_UNSUPPORTED, "%s: %lld tiles per sequence", what, per_seq);
+    }
+    for (int b0 = 0; b0 < batch; b0 += chunk) {
+        a.batch = std::min(chunk, batch - b0);
         a.tables = block_tables + (int64_t)b0 * max_blocks_per_seq;
         a.ctx_lens = ctx_lens + b0;
         a.q = (const char*)q + b0 * q_stride * size;
