@@ -259,28 +259,49 @@ __global__ __launch_bounds__(256) void kv8_write_kernel(Kv8WriteArgs a) {
     const long long r1 = min(r0 + a.span, (long long)a.n_rows);
     bool bad = false;
     const auto inside = [&](long long slot) { return slot >= 0 && slot < end; };
-    for (long long r = r0; r < r1; r++) {
-        {
-            const long long back = r - lane >= 0 ? a.slots[r - lane] : -1;
-            const unsigned long long any = __ballot(inside(back));
-            if (!(any & 1)) continue;  // skipped
-            const unsigned long long rest = any & ~1ull;
-            const int at_prev = rest ? (int)__builtin_ctzll(rest) : 0;
-            const int mine = (int)(back >> a.c.bt_log2);
-            if (rest && __builtin_amdgcn_readlane(mine, at_prev) == __builtin_amdgcn_readlane(mine, 0))
-                continue;  // not the block's first row
-        }
-        for (bool more = true; more;) {
-            const long long slot = a.slots[r];
+    // the first rows of blocks among the span's, all at once: a lane looks at
+    // one row and at the last row before it that is not skipped
+    const long long cur = r0 + lane < a.n_rows ? a.slots[r0 + lane] : -1;
+    const long long prev = r0 - 64 + lane >= 0 ? a.slots[r0 - 64 + lane] : -1;
+    unsigned long long firsts;
+    {
+        const unsigned long long on = __ballot(inside(cur)), before = __ballot(inside(prev));
+        const unsigned long long below = on & ((1ull << lane) - 1);
+        const int mine = (int)(cur >> a.c.bt_log2);
+        const int last = before ? 63 - (int)__builtin_clzll(before) : 0;
+        const int last_block = __builtin_amdgcn_readlane((int)(prev >> a.c.bt_log2), last);
+        const int near_block = __shfl(mine, below ? 63 - (int)__builtin_clzll(below) : 0);
+        const bool follows = below ? near_block == mine : before && lane + 64 - last < 64 && last_block == mine;
+        firsts = __ballot(inside(cur) && lane < r1 - r0 && !follows);
+    }
+    for (; firsts; firsts &= firsts - 1) {
+        const int i0 = (int)__builtin_ctzll(firsts);
+        long long r = r0 + i0;
+        bool in_window = true;
+        for (bool more = true; more; in_window = false) {
+            long long slot;
+            if (in_window) {
+                const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)cur, i0);
+                const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(cur >> 32), i0);
+                slot = (long long)(((unsigned long long)hi << 32) | lo);
+            } else {
+                slot = a.slots[r];
+            }
             const int place = (int)(slot & (bt - 1));
             // the run's length
             const int most = (int)min((long long)(bt - place), a.n_rows - r);
-            int n = 1;
-            for (int i = 0; i < most; i += 64) {
-                const bool on = i + lane < most && a.slots[r + i + lane] == slot + i + lane;
-                const unsigned long long off = ~__ballot(on);
-                n = i + (off ? (int)__builtin_ctzll(off) : 64);
-                if (off) break;
+            int n = 0;
+            if (in_window) {  // from the rows that are here already
+                const unsigned long long on = __ballot(lane >= i0 && cur == slot + (lane - i0)) >> i0;
+                n = min(~on ? (int)__builtin_ctzll(~on) : 64, most);
+            }
+            if (!in_window || (i0 + n == 64 && n < most)) {
+                for (int i = n; i < most; i += 64) {
+                    const bool on = i + lane < most && a.slots[r + i + lane] == slot + i + lane;
+                    const unsigned long long off = ~__ballot(on);
+                    n = i + (off ? (int)__builtin_ctzll(off) : 64);
+                    if (off) break;
+                }
             }
             // what follows it, requested ahead of the rows
             const long long next = r + n + lane < a.n_rows ? a.slots[r + n + lane] : -1;

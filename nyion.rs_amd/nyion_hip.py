@@ -238,9 +238,15 @@ def check(rc: int, what: str = "") -> None:
 # torch helpers
 # ----------------------------------------------------------------------------
 
+_torch_module = None
+
+
 def _torch():
-    import torch
-    return torch
+    global _torch_module
+    if _torch_module is None:
+        import torch
+        _torch_module = torch
+    return _torch_module
 
 
 def ptr(t) -> int | None:
@@ -620,31 +626,38 @@ def _want(ok, what: str) -> None:
         raise NyionError(ERR_INVALID, what)
 
 
-def _on_current_device(*tensors) -> bool:
+# The calls below check their tensors and are as short as the work they launch (4 us for a batch
+# map), so the checks are attribute comparisons, without a message until one fails.
+
+def _current_device() -> int:
     torch = _torch()
-    dev = torch.cuda.current_device()
-    return all(t is None or (t.is_cuda and t.get_device() == dev) for t in tensors)
+    get = getattr(torch._C, "_cuda_getDevice", None)
+    return get() if get is not None and torch.cuda.is_initialized() else torch.cuda.current_device()
+
+
+def _check_packed(dtype, device, *tensors) -> None:
+    """Contiguous tensors of one type on one device."""
+    for t in tensors:
+        if t.dtype is not dtype or t.get_device() != device or not t.is_contiguous():
+            raise NyionError(ERR_INVALID, f"a contiguous {dtype} tensor on device {device} is "
+                             f"wanted, not {t.dtype} {tuple(t.shape)} {t.stride()} on {t.device}")
+
+
+def _check_rows(t, heads, head_dim, device) -> None:
+    """[rows][heads][head_dim], rows any distance apart."""
+    shape, stride = t.shape, t.stride()
+    if (len(shape) != 3 or shape[1] != heads or shape[2] != head_dim or stride[2] != 1
+            or stride[1] != head_dim and heads != 1 or t.get_device() != device):
+        raise NyionError(ERR_INVALID, f"[rows][{heads}][{head_dim}] with contiguous rows on device "
+                         f"{device} is wanted, not {tuple(shape)} {stride} on {t.device}")
 
 
 def _io_dtype(t) -> int:
     torch = _torch()
-    if t.dtype == torch.float32:
+    if t.dtype is torch.float32:
         return IO_F32
-    _want(t.dtype == torch.bfloat16, f"rows are float32 or bfloat16, not {t.dtype}")
+    _want(t.dtype is torch.bfloat16, f"rows are float32 or bfloat16, not {t.dtype}")
     return IO_BF16
-
-
-def _check_rows(t, heads, head_dim, what) -> None:
-    """[rows][heads][head_dim], rows any distance apart."""
-    _want(t.dim() == 3 and t.shape[1] == heads and t.shape[2] == head_dim,
-          f"{what} is [rows][{heads}][{head_dim}], not {tuple(t.shape)}")
-    s = t.stride()
-    _want(s[2] == 1 and (s[1] == head_dim or heads == 1), f"{what}: a row is contiguous")
-
-
-def _check_int(t, torch_dtype, what, n=None) -> None:
-    _want(t.dtype == torch_dtype and t.is_contiguous(), f"{what} is contiguous {torch_dtype}")
-    _want(n is None or t.numel() == n, f"{what} has {n} entries, not {t.numel()}")
 
 
 class Kv8Cache:
@@ -676,9 +689,13 @@ class Kv8Cache:
         ks, vs = (torch.zeros(shape[:2], dtype=torch.float32, device=device) for _ in range(2))
         return cls(k, v, ks, vs, code)
 
-    def check_device(self) -> None:
-        _want(self.device_index == _torch().cuda.current_device(),
-              "the cache is on another device than the current one")
+    def device_now(self) -> int:
+        """The current device, which has to be the cache's."""
+        device = _current_device()
+        if self.device_index != device:
+            raise NyionError(ERR_INVALID, f"the cache is on device {self.device_index}, the current "
+                             f"one is {device}")
+        return device
 
 
 class ScoreOptions:
@@ -688,21 +705,18 @@ class ScoreOptions:
     def __init__(self, scale=0.0, softcap=0.0, window=0, slopes=None, prefix_lens=None):
         torch = _torch()
         if slopes is not None:
-            _want(slopes.dtype == torch.float32 and slopes.is_contiguous(),
-                  "slopes are contiguous float32")
+            _check_packed(torch.float32, slopes.get_device(), slopes)
         if prefix_lens is not None:
-            _check_int(prefix_lens, torch.int32, "prefix_lens")
+            _check_packed(torch.int32, prefix_lens.get_device(), prefix_lens)
         self.slopes, self.prefix_lens, self.window = slopes, prefix_lens, window
         self.struct = ScoreOptionsStruct(scale, softcap, window, 0, ptr(slopes), ptr(prefix_lens))
         self.ref = C.addressof(self.struct)
 
-    def check(self, n_heads, batch) -> None:
-        _want(self.slopes is None or self.slopes.numel() == n_heads,
-              f"slopes have {n_heads} entries")
-        _want(self.prefix_lens is None or self.prefix_lens.numel() == batch,
-              f"prefix_lens have {batch} entries")
-        _want(_on_current_device(self.slopes, self.prefix_lens),
-              "the options' tensors are on the current device")
+    def check(self, n_heads, batch, device) -> None:
+        for t, n in ((self.slopes, n_heads), (self.prefix_lens, batch)):
+            if t is not None and (t.numel() != n or t.get_device() != device):
+                raise NyionError(ERR_INVALID, f"slopes and prefix_lens have one entry for each of "
+                                 f"{n_heads} heads and {batch} sequences, on device {device}")
 
 
 def batch_map(cached_lens, new_lens, free_blocks, block_tables, block_tokens, num_blocks, ctx_lens,
@@ -711,36 +725,42 @@ def batch_map(cached_lens, new_lens, free_blocks, block_tables, block_tokens, nu
     block_tables [B][max_blocks] (updated) int32; written: ctx_lens [B], row_starts [B + 1],
     positions [n_rows], counts [2] int32 and slots [n_rows] int64."""
     torch = _torch()
-    B = cached_lens.numel()
-    for t, what, n in ((cached_lens, "cached_lens", B), (new_lens, "new_lens", B),
-                       (free_blocks, "free_blocks", None), (ctx_lens, "ctx_lens", B),
-                       (block_tables, "block_tables", None), (row_starts, "row_starts", B + 1),
-                       (positions, "positions", slots.numel()), (counts, "counts", 2)):
-        _check_int(t, torch.int32, what, n)
-    _check_int(slots, torch.int64, "slots")
-    _want(block_tables.dim() == 2 and block_tables.shape[0] == B, f"block_tables is [{B}][blocks]")
-    _want(_on_current_device(cached_lens, new_lens, free_blocks, block_tables, ctx_lens, row_starts,
-                             slots, positions, counts), "tensors are on the current device")
+    B, n_rows, tables = cached_lens.numel(), slots.numel(), block_tables.shape
+    device = _current_device()
+    _check_packed(torch.int32, device, cached_lens, new_lens, free_blocks, block_tables, ctx_lens,
+                  row_starts, positions, counts)
+    _check_packed(torch.int64, device, slots)
+    if (new_lens.numel() != B or ctx_lens.numel() != B or row_starts.numel() != B + 1
+            or positions.numel() != n_rows or counts.numel() != 2 or len(tables) != 2
+            or tables[0] != B):
+        raise NyionError(ERR_INVALID, f"for {B} sequences and {n_rows} rows: new_lens and ctx_lens "
+                         f"[{B}], row_starts [{B + 1}], positions [{n_rows}], counts [2], "
+                         f"block_tables [{B}][blocks]")
     rc = load().nyion_batch_map(
-        ptr(cached_lens), ptr(new_lens), B, ptr(free_blocks), free_blocks.numel(), block_tokens,
-        num_blocks, ptr(block_tables), block_tables.shape[1], ptr(ctx_lens), ptr(row_starts),
-        ptr(slots), ptr(positions), slots.numel(), ptr(counts), stream_handle(stream))
-    check(rc, "nyion_batch_map")
+        cached_lens.data_ptr(), new_lens.data_ptr(), B, free_blocks.data_ptr(),
+        free_blocks.numel(), block_tokens, num_blocks, block_tables.data_ptr(), tables[1],
+        ctx_lens.data_ptr(), row_starts.data_ptr(), slots.data_ptr(), positions.data_ptr(), n_rows,
+        counts.data_ptr(), stream_handle(stream))
+    if rc:
+        check(rc, "nyion_batch_map")
 
 
 def kv8_write(cache, slots, k, v, stream=None):
     """Rows k, v [n_rows][Hkv][D] (f32 or bf16, rows any distance apart) into the cache at
     slots [n_rows] int64, as batch_map gives them."""
     torch = _torch()
-    cache.check_device()
-    for t, what in ((k, "k"), (v, "v")):
-        _check_rows(t, cache.n_kv_heads, cache.head_dim, what)
-    _want(k.dtype == v.dtype and k.shape == v.shape, "k and v are alike")
-    _check_int(slots, torch.int64, "slots", k.shape[0])
-    _want(_on_current_device(slots, k, v), "tensors are on the current device")
-    rc = load().nyion_kv8_write(cache.ref, ptr(slots), k.shape[0], ptr(k), k.stride(0), ptr(v),
-                                v.stride(0), _io_dtype(k), stream_handle(stream))
-    check(rc, "nyion_kv8_write")
+    device = cache.device_now()
+    _check_rows(k, cache.n_kv_heads, cache.head_dim, device)
+    _check_rows(v, cache.n_kv_heads, cache.head_dim, device)
+    _check_packed(torch.int64, device, slots)
+    n_rows = slots.numel()
+    if k.dtype is not v.dtype or k.shape[0] != n_rows or v.shape[0] != n_rows:
+        raise NyionError(ERR_INVALID, f"k and v are of one type and have {n_rows} rows, one for "
+                         "each slot")
+    rc = load().nyion_kv8_write(cache.ref, slots.data_ptr(), n_rows, k.data_ptr(), k.stride(0),
+                                v.data_ptr(), v.stride(0), _io_dtype(k), stream_handle(stream))
+    if rc:
+        check(rc, "nyion_kv8_write")
 
 
 def kv8_decode_workspace_size(cache, batch, n_heads, max_ctx, window=0) -> int:
@@ -748,39 +768,49 @@ def kv8_decode_workspace_size(cache, batch, n_heads, max_ctx, window=0) -> int:
 
 
 def _check_attention(cache, q, block_tables, ctx_lens, out, options):
+    """(q heads, sequences, current device) of a call whose tensors fit each other."""
     torch = _torch()
-    cache.check_device()
-    n_heads, B = q.shape[1], ctx_lens.numel()
-    _check_rows(q, n_heads, cache.head_dim, "q")
-    _want(out.shape == q.shape and out.dtype == q.dtype and out.is_contiguous(),
-          "out is contiguous and has q's shape and type")
-    _check_int(ctx_lens, torch.int32, "ctx_lens")
-    _check_int(block_tables, torch.int32, "block_tables")
-    _want(block_tables.dim() == 2 and block_tables.shape[0] == B, f"block_tables is [{B}][blocks]")
-    _want(_on_current_device(q, block_tables, ctx_lens, out), "tensors are on the current device")
+    device = cache.device_now()
+    n_heads, B, tables = q.shape[1], ctx_lens.numel(), block_tables.shape
+    _check_rows(q, n_heads, cache.head_dim, device)
+    _check_packed(torch.int32, device, ctx_lens, block_tables)
+    _check_packed(q.dtype, device, out)
+    if out.shape != q.shape or len(tables) != 2 or tables[0] != B:
+        raise NyionError(ERR_INVALID, f"out has q's shape {tuple(q.shape)}, block_tables is "
+                         f"[{B}][blocks]")
     if options is not None:
-        options.check(n_heads, B)
-    return n_heads, B
+        options.check(n_heads, B, device)
+    return n_heads, B, device
 
 
 def kv8_decode(cache, q, block_tables, ctx_lens, out, max_ctx=None, options=None, workspace=None,
                stream=None):
     """Attention of one row per sequence over the cache: q, out [B][Hq][D] f32 or bf16,
     block_tables [B][max_blocks], ctx_lens [B] int32.  Returns the workspace."""
-    n_heads, B = _check_attention(cache, q, block_tables, ctx_lens, out, options)
-    _want(q.shape[0] == B, f"q has {B} rows")
+    n_heads, B, device = _check_attention(cache, q, block_tables, ctx_lens, out, options)
+    if q.shape[0] != B:
+        raise NyionError(ERR_INVALID, f"q has {q.shape[0]} rows for {B} sequences")
     if max_ctx is None:
         max_ctx = max(int(ctx_lens.max().item()), 1)
     if workspace is None:
         workspace = alloc_workspace(kv8_decode_workspace_size(
             cache, B, n_heads, max_ctx, 0 if options is None else options.window), q.device)
-    ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
+    ws, ws_bytes = _workspace_args(workspace, device)
     rc = load().nyion_kv8_decode_attention(
-        cache.ref, ptr(block_tables), block_tables.shape[1], ptr(ctx_lens), B, max_ctx, ptr(q),
-        q.stride(0), ptr(out), n_heads, _io_dtype(q), None if options is None else options.ref,
-        ptr(workspace), ws_bytes, stream_handle(stream))
-    check(rc, "nyion_kv8_decode_attention")
+        cache.ref, block_tables.data_ptr(), block_tables.shape[1], ctx_lens.data_ptr(), B, max_ctx,
+        q.data_ptr(), q.stride(0), out.data_ptr(), n_heads, _io_dtype(q),
+        None if options is None else options.ref, ws, ws_bytes, stream_handle(stream))
+    if rc:
+        check(rc, "nyion_kv8_decode_attention")
     return workspace
+
+
+def _workspace_args(workspace, device):
+    if workspace is None:
+        return None, 0
+    if workspace.get_device() != device:
+        raise NyionError(ERR_INVALID, f"the workspace is on {workspace.device}, not on {device}")
+    return workspace.data_ptr(), workspace.numel() * workspace.element_size()
 
 
 def kv8_prefill_workspace_size(cache, batch, n_heads, n_rows, max_rows, max_ctx, window=0) -> int:
@@ -793,10 +823,10 @@ def kv8_prefill_bf16(cache, q, block_tables, ctx_lens, row_starts, out, max_rows
     """Attention of a ragged batch over the cache: q, out [n_rows][Hq][D] bf16, the rows of sequence
     b, row_starts [B + 1] int32, being its last tokens.  Returns the workspace."""
     torch = _torch()
-    n_heads, B = _check_attention(cache, q, block_tables, ctx_lens, out, options)
-    _want(q.dtype == torch.bfloat16, f"q is bfloat16, not {q.dtype}")
-    _check_int(row_starts, torch.int32, "row_starts", B + 1)
-    _want(_on_current_device(row_starts), "row_starts is on the current device")
+    n_heads, B, device = _check_attention(cache, q, block_tables, ctx_lens, out, options)
+    _check_packed(torch.int32, device, row_starts)
+    if q.dtype is not torch.bfloat16 or row_starts.numel() != B + 1:
+        raise NyionError(ERR_INVALID, f"q is bfloat16, not {q.dtype}; row_starts has {B + 1} entries")
     n_rows = q.shape[0]
     if max_rows is None:
         max_rows = max(int((row_starts[1:] - row_starts[:-1]).max().item()), 1)
@@ -806,12 +836,14 @@ def kv8_prefill_bf16(cache, q, block_tables, ctx_lens, row_starts, out, max_rows
         workspace = alloc_workspace(kv8_prefill_workspace_size(
             cache, B, n_heads, n_rows, max_rows, max_ctx, 0 if options is None else options.window),
             q.device)
-    ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
+    ws, ws_bytes = _workspace_args(workspace, device)
     rc = load().nyion_kv8_prefill_attention_bf16(
-        cache.ref, ptr(block_tables), block_tables.shape[1], ptr(ctx_lens), ptr(row_starts), B,
-        n_rows, max_rows, max_ctx, ptr(q), q.stride(0), ptr(out), n_heads,
-        None if options is None else options.ref, ptr(workspace), ws_bytes, stream_handle(stream))
-    check(rc, "nyion_kv8_prefill_attention_bf16")
+        cache.ref, block_tables.data_ptr(), block_tables.shape[1], ctx_lens.data_ptr(),
+        row_starts.data_ptr(), B, n_rows, max_rows, max_ctx, q.data_ptr(), q.stride(0),
+        out.data_ptr(), n_heads, None if options is None else options.ref, ws, ws_bytes,
+        stream_handle(stream))
+    if rc:
+        check(rc, "nyion_kv8_prefill_attention_bf16")
     return workspace
 
 

@@ -222,6 +222,21 @@ def test_write_reports_what_is_not_finite(gpu, code):
     assert gpu.take_status()[0] == gpu.OK
 
 
+@pytest.mark.parametrize("bt", [16, 64, 256])
+def test_write_of_runs_that_windows_cut(gpu, bt):
+    """Runs across the 64 rows that a wavefront sees at once, blocks that follow each other in the
+    cache, several runs of one block with skipped rows between them, at every phase."""
+    rng = np.random.default_rng(bt)
+    for lead in (0, 1, 37, 63, 64, 65):
+        slots = [-1] * lead + list(range(5, 5 + 3 * bt)) + [-1] * 62 + [3 * bt + 9, 3 * bt + 10]
+        slots += [6 * bt, 6 * bt + 1, -1, -1, 6 * bt + 7, 6 * bt + 3, 6 * bt + 4, 2 ** 40, 8 * bt + bt - 1]
+        x = rng.standard_normal((2, len(slots), 1, 64)) * np.exp(rng.standard_normal((2, len(slots), 1, 1)))
+        run_write(gpu, E4M3 if lead % 2 else INT8, 10, 1, bt, 64, slots, x, "f32", seed=lead)
+    slots = [s for b in rng.permutation(300) for s in range(b * bt, b * bt + bt)] if bt == 16 else list(range(9 * bt))
+    x = rng.standard_normal((2, len(slots), 4, 64))
+    run_write(gpu, E4M3, 300 if bt == 16 else 9, 4, bt, 64, slots, x, "bf16")
+
+
 def test_write_skips_slots_outside_the_cache(gpu):
     rng = np.random.default_rng(10)
     slots = [-1, 5, 6, 64, 2 ** 40, -2 ** 40, 63, 7, 8]
