@@ -3,8 +3,8 @@
 // Sequence b brings rows_b query rows, the last tokens of its context, and
 // each kv head is read by `group` q heads.  The rows_b * group (row, head)
 // pairs of a kv head are numbered row-major, whatever the group's size, and cut
-// into tiles; a workgroup of four wavefronts takes one tile of 128 * NT pairs,
-// 32 * NT a wavefront, through the keys that its rows see, 64 at a time:
+// into tiles; a workgroup of four wavefronts takes one tile of 128 pairs, 32 a
+// wavefront, through the keys that its rows see, 64 at a time:
 //   S^T[32 keys][32 pairs] += K . Q^T    v_mfma_f32_32x32x16_f16
 //   O^T[32 dims][32 pairs] += V^T . P^T  v_mfma_f32_32x32x16_f16
 // The result layout of S^T (a lane holds one pair and 16 keys) is the B
@@ -24,7 +24,7 @@
 // of a tile wait for nothing but LDS; longer ranges refill it.
 //
 // Weights are binary16 against a running maximum that moves only when a sum
-// of 16 weights passes 2^14; q is binary16 relative to its row's largest value.
+// of 32 weights passes 2^14; q is binary16 relative to its row's largest value.
 //
 // Few tiles: their keys are cut into pieces as well, joined through the
 // workspace by the last piece to arrive, in the order of the pieces.
@@ -38,8 +38,12 @@
 namespace nyion {
 
 constexpr int kKeys = 64;          // per tile
+constexpr int kWavePairs = 32;     // pairs per wavefront
 constexpr int kTableTiles = 128;   // tiles of the page table in LDS
 constexpr int kSeqsMax = 1024;     // sequences per launch
+constexpr int kSorted = 512;       // tiles of a kv head that are put in order of their lengths
+constexpr int kPieceTiles = 4;   // fewest tiles of a piece
+constexpr int kMaxPieces = 16;   // the join walks them one by one
 constexpr float kSumLimit = 16384.f;
 constexpr float kVUnit = 64.f;     // 448 * 64 stays below binary16's largest
 constexpr float kVLeast = 7.888609052210118e-31f;  // 2^-100
@@ -63,7 +67,6 @@ struct Kv8PrefillArgs {
     int n_heads;
     int group;
     int pieces;
-    int min_tiles;
     int max_items;  // (tile, kv head)s that the launch and the workspace hold
 };
 
@@ -75,10 +78,11 @@ struct Kv8Lds {
     static constexpr int VBYTES = D * VROW;
     static constexpr int TILES = 2 * (KBYTES + VBYTES);
     static constexpr int SUBS = 4 * kTableTiles;
-    static constexpr int OFF = TILES;               // long long [SUBS]
+    static constexpr int OFF = TILES;               // long long [SUBS]: bytes; 0 where absent
     static constexpr int KS = OFF + SUBS * 8;       // float [SUBS]
     static constexpr int VS = KS + SUBS * 4;        // float [SUBS]
-    static constexpr int MISC = VS + SUBS * 4;      // int [16]
+    static constexpr int GONE = VS + SUBS * 4;      // uint32 [SUBS / 32]: bits of absent subtiles
+    static constexpr int MISC = GONE + SUBS / 8;    // int [16]
     static constexpr int BYTES = MISC + 64;
 };
 
@@ -91,18 +95,49 @@ __device__ __forceinline__ float sum_half(float v) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-template <int D, int CODE, bool MODS, int NT>
-__global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void kv8_prefill_kernel(Kv8PrefillArgs a) {
+// The keys that a tile of pairs sees, as tiles of kKeys.
+struct PairSpan {
+    int row0, rows;  // of the sequence
+    int live;        // its keys that can be read
+    int pos0;        // position of its row 0
+    int prefix;
+    int tile0, tiles;
+};
+__device__ __forceinline__ PairSpan pair_span(const Kv8PrefillArgs& a, int b, int tile, int tm) {
+    PairSpan r;
+    r.row0 = min(max(a.row_starts[b], 0), a.n_rows);
+    r.rows = min(max(a.row_starts[b + 1], r.row0), a.n_rows) - r.row0;
+    const int ctx = a.ctx_lens[b];
+    r.live = max(min(ctx, a.span), 0);
+    r.pos0 = ctx - r.rows;
+    r.prefix = a.s.prefix_lens ? a.s.prefix_lens[b] : 0;
+    const int last_pair = min(tile * tm + tm, r.rows * a.group) - 1;
+    const int first = r.pos0 + tile * tm / a.group, last = r.pos0 + last_pair / a.group;
+    const int end = last < 0 ? 0 : min(max(last + 1, r.prefix), r.live);
+    const int begin = a.s.window > 0 ? min(max(first - a.s.window + 1, 0), end) : 0;
+    r.tile0 = begin / kKeys;
+    r.tiles = (end + kKeys - 1) / kKeys - r.tile0;
+    return r;
+}
+
+template <int D, int CODE, bool CAP, bool BIAS, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, 2 * 4 / WAVES) void kv8_prefill_kernel(Kv8PrefillArgs a) {
     using L = Kv8Lds<D>;
     constexpr int DT = D / 32;       // 32-dim tiles of O^T
     constexpr int KS = D / 16;       // k-steps of the S product
-    constexpr int TM = 128 * NT;     // (row, head) pairs per workgroup
-    constexpr int KL = D / 64;       // 16-byte K chunks per thread and tile
-    constexpr int VL = D / 64;       // V units per thread and tile
+    constexpr int NT = 64 * WAVES;
+    constexpr bool PHASES = WAVES == 8;
+    constexpr int TM = kWavePairs * WAVES;  // (row, head) pairs per workgroup
+    // K chunks of 16 bytes and V units of 4 tokens by 4 dims, D * 4 of each a
+    // tile: with fewer than threads, one half stages K and the other V
+    constexpr bool APART = 4 * D < NT;
+    constexpr int KL = APART ? 1 : 4 * D / NT;
+    constexpr int VL = KL;
     __shared__ __attribute__((aligned(16))) unsigned char lds[L::BYTES];
-    long long* const sub_off = (long long*)(lds + L::OFF);  // -1: absent
+    long long* const sub_off = (long long*)(lds + L::OFF);
     float* const sub_ks = (float*)(lds + L::KS);
     float* const sub_vs = (float*)(lds + L::VS);
+    uint32_t* const sub_gone = (uint32_t*)(lds + L::GONE);
     int* const misc = (int*)(lds + L::MISC);
 
     const int tid = threadIdx.x;
@@ -110,14 +145,16 @@ __global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void kv8_prefill_kernel(Kv8Pr
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int j = lane & 31;
     const int h = lane >> 5;
+    const bool second = wave >= WAVES / 2;  // half of the workgroup, a phase behind the other
 
     // ---- this workgroup's sequence, kv head, tile of pairs and piece
     int b = 0, tile = 0, kvh = 0, piece = 0;
-    long long item;
+    int item;
+    const auto span_of = [&](int b, int tile) { return pair_span(a, b, tile, TM); };
     {
         int* const ends = (int*)lds;  // tiles up to and with each sequence
         int before = 0;
-        for (int b0 = 0; b0 < a.batch; b0 += 256) {
+        for (int b0 = 0; b0 < a.batch; b0 += NT) {
             const int s = b0 + tid;
             int x = 0;
             if (s < a.batch) {
@@ -134,7 +171,7 @@ __global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void kv8_prefill_kernel(Kv8Pr
             __syncthreads();
             int all = 0;
 #pragma unroll
-            for (int w = 0; w < 4; w++) {
+            for (int w = 0; w < WAVES; w++) {
                 if (w < wave) x += misc[w];
                 all += misc[w];
             }
@@ -145,65 +182,81 @@ __global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void kv8_prefill_kernel(Kv8Pr
         const int tiles = __builtin_amdgcn_readfirstlane(before);
         // an XCD (workgroup id mod 8) takes a run of the list (kv head, tile,
         // piece): its L2 then holds few heads' keys
-        const long long items = (long long)tiles * a.c.n_kv_heads * a.pieces;
-        const long long per = (items + 7) / 8;
-        const long long at = (int)(blockIdx.x >> 3);
-        item = (blockIdx.x & 7) * per + at;
-        if (at >= per || item >= items || item / a.pieces >= a.max_items) return;
-        const int per_head = tiles * a.pieces;
-        kvh = (int)(item / per_head);
-        const int rest = (int)(item - (long long)kvh * per_head);
-        const int t = tiles - 1 - rest / a.pieces;  // later tiles of a sequence are longer: first
-        piece = rest % a.pieces;
-        int lo = 0, hi = a.batch - 1;
-        while (lo < hi) {
-            const int mid = (lo + hi) >> 1;
-            if (ends[mid] > t)
-                hi = mid;
-            else
-                lo = mid + 1;
+        const uint32_t items = min((uint64_t)tiles * a.c.n_kv_heads, (uint64_t)a.max_items) * a.pieces;
+        const uint32_t per = (items + 7) / 8, at = blockIdx.x >> 3;
+        const uint32_t mine = (blockIdx.x & 7) * per + at;
+        if (at >= per || mine >= items) return;
+        // counters and partials go by (kv head, tile)
+        item = (int)(mine / a.pieces);
+        piece = (int)mine - item * a.pieces;
+        kvh = item / tiles;
+        const int place = item - kvh * tiles;
+        const auto sequence_of = [&](int t) {
+            int lo = 0, hi = a.batch - 1;
+            while (lo < hi) {
+                const int mid = (lo + hi) >> 1;
+                if (ends[mid] > t)
+                    hi = mid;
+                else
+                    lo = mid + 1;
+            }
+            return lo;
+        };
+        int t = tiles - 1 - place;  // later tiles of a sequence are longer: first
+        if (a.batch > 1 && tiles <= kSorted) {
+            // several sequences: the longest of all first (a batch of nine, 1-900 rows
+            // behind up to 2000 tokens: 200 -> 183 us)
+            int* const length = (int*)lds + kSeqsMax;  // [tiles], zeros to a multiple of 4
+            const int n4 = (tiles + 3) & ~3;
+            for (int i = tid; i < n4; i += NT) {
+                int n = 0;
+                if (i < tiles) {
+                    const int s = sequence_of(i);
+                    n = span_of(s, i - (s > 0 ? ends[s - 1] : 0)).tiles + 1;
+                }
+                length[i] = n;
+            }
+            __syncthreads();
+            for (int i = tid; i < tiles; i += NT) {
+                const int mine = length[i];
+                int rank = 0;
+                for (int k = 0; k < n4; k += 4) {
+                    const int4 n = *(const int4*)(length + k);
+                    rank += (n.x > mine || (n.x == mine && k < i)) + (n.y > mine || (n.y == mine && k + 1 < i)) +
+                            (n.z > mine || (n.z == mine && k + 2 < i)) + (n.w > mine || (n.w == mine && k + 3 < i));
+                }
+                if (rank == place) misc[9] = i;
+            }
+            __syncthreads();
+            t = misc[9];
         }
-        b = __builtin_amdgcn_readfirstlane(lo);
+        b = __builtin_amdgcn_readfirstlane(sequence_of(t));
         tile = __builtin_amdgcn_readfirstlane(t - (b > 0 ? ends[b - 1] : 0));
-        // counters and partials go by (sequence's tile, head): item / pieces
-        item = item / a.pieces;
         __syncthreads();
     }
-    const int row0 = min(max(a.row_starts[b], 0), a.n_rows);
-    const int rows = min(max(a.row_starts[b + 1], row0), a.n_rows) - row0;
-    const int ctx = a.ctx_lens[b];
-    const int live = max(min(ctx, a.span), 0);  // keys that can be read
-    const int pos0 = ctx - rows;                // position of row 0
-    const int prefix = a.s.prefix_lens ? a.s.prefix_lens[b] : 0;
+    const PairSpan sp = span_of(b, tile);
+    const int row0 = sp.row0, rows = sp.rows, live = sp.live, pos0 = sp.pos0, prefix = sp.prefix;
     const int pairs = rows * a.group;
     const int32_t* table = a.tables + (long long)b * a.max_blocks;
-
-    // ---- keys of the tile's rows
-    const int i_first = tile * TM / a.group;
-    const int i_last = min(tile * TM + TM, pairs) - 1;
-    const int p_first = pos0 + i_first, p_last = pos0 + i_last / a.group;
-    const int key_end = p_last < 0 ? 0 : min(max(p_last + 1, prefix), live);
-    const int key_begin = a.s.window > 0 ? min(max(p_first - a.s.window + 1, 0), key_end) : 0;
-    const int tile0 = key_begin / kKeys;
-    const int all_tiles = (key_end + kKeys - 1) / kKeys - tile0;
-    const int n_pieces = max(min(a.pieces, all_tiles / a.min_tiles), 1);
+    const int n_pieces = max(min(a.pieces, sp.tiles / kPieceTiles), 1);
     if (piece >= n_pieces) return;
-    const int t_first = tile0 + (int)((long long)all_tiles * piece / n_pieces);
-    const int n_tiles = tile0 + (int)((long long)all_tiles * (piece + 1) / n_pieces) - t_first;
+    // pieces of tiles / n_pieces, the first ones one more
+    const int part = sp.tiles / n_pieces, more = sp.tiles - part * n_pieces;
+    const int t_first = sp.tile0 + part * piece + min(piece, more);
+    const int n_tiles = part + (piece < more ? 1 : 0);
 
-    // ---- the pairs of this lane: q, bounds
-    half8_t qreg[NT][KS];
-    float crow[NT], slope[NT];
-    int key_lo[NT], key_hi[NT], qpos[NT];
-#pragma unroll
-    for (int t = 0; t < NT; t++) {
-        const int x = min(tile * TM + (wave * NT + t) * 32 + j, pairs - 1);
+    // ---- the pair of this lane: q, bounds
+    half8_t qreg[KS];
+    float crow, slope;
+    int key_lo, key_hi, qpos;
+    {
+        const int x = min(tile * TM + wave * kWavePairs + j, pairs - 1);
         const int i = x / a.group;
         const int head = kvh * a.group + (x - i * a.group);
-        qpos[t] = pos0 + i;
-        key_hi[t] = qpos[t] < 0 ? 0 : min(max(qpos[t] + 1, prefix), live);  // exclusive
-        key_lo[t] = a.s.window > 0 ? max(qpos[t] - a.s.window + 1, 0) : 0;
-        slope[t] = MODS && a.s.slopes ? a.s.slopes[head] * 1.4426950408889634f : 0.f;
+        qpos = pos0 + i;
+        key_hi = qpos < 0 ? 0 : min(max(qpos + 1, prefix), live);  // exclusive
+        key_lo = a.s.window > 0 ? max(qpos - a.s.window + 1, 0) : 0;
+        slope = BIAS ? a.s.slopes[head] * 1.4426950408889634f : 0.f;
         const uint16_t* qrow = a.q + (long long)(row0 + i) * a.q_stride + head * D + 8 * h;
         u32x4_t w[KS];
         float top = 0.f;
@@ -222,45 +275,43 @@ __global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void kv8_prefill_kernel(Kv8Pr
         for (int s = 0; s < KS; s++)
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                qreg[t][s][2 * e] = (_Float16)__builtin_amdgcn_ldexpf(__uint_as_float(w[s][e] << 16), -ex);
-                qreg[t][s][2 * e + 1] = (_Float16)__builtin_amdgcn_ldexpf(__uint_as_float(w[s][e] & 0xffff0000u), -ex);
+                qreg[s][2 * e] = (_Float16)__builtin_amdgcn_ldexpf(__uint_as_float(w[s][e] << 16), -ex);
+                qreg[s][2 * e + 1] = (_Float16)__builtin_amdgcn_ldexpf(__uint_as_float(w[s][e] & 0xffff0000u), -ex);
             }
-        crow[t] = __builtin_amdgcn_ldexpf(a.s.scale_log2, ex);
+        crow = __builtin_amdgcn_ldexpf(a.s.scale_log2, ex);
     }
     // bounds of the wavefront's pairs together, for whole tiles
     int w_lo = 0, w_hi = 0;
     {
-        const int x0 = min(tile * TM + wave * NT * 32, pairs - 1) / a.group;
-        const int x1 = min(tile * TM + (wave * NT + NT) * 32 - 1, pairs - 1) / a.group;
+        const int x0 = min(tile * TM + wave * kWavePairs, pairs - 1) / a.group;
+        const int x1 = min(tile * TM + wave * kWavePairs + kWavePairs - 1, pairs - 1) / a.group;
         w_hi = pos0 + x0 < 0 ? 0 : min(max(pos0 + x0 + 1, prefix), live);   // smallest end
         w_lo = a.s.window > 0 ? max(pos0 + x1 - a.s.window + 1, 0) : 0;      // largest begin
     }
 
-    float16_t o[NT][DT];
-    float mrun[NT], lrun[NT];
+    float16_t o[DT];
 #pragma unroll
-    for (int t = 0; t < NT; t++) {
-#pragma unroll
-        for (int d = 0; d < DT; d++) o[t][d] = float16_t{};
-        mrun[t] = -1e30f;  // finite: exp2(-inf - mrun) is 0, never NaN
-        lrun[t] = 0.f;
-    }
+    for (int d = 0; d < DT; d++) o[d] = float16_t{};
+    float mrun = -1e30f;  // finite: exp2(-inf - mrun) is 0, never NaN
+    float lrun = 0.f;
 
     // ---- the page table of nt tiles from tile t0 on; returns the largest V scale
     auto fill = [&](int t0, int nt) __attribute__((always_inline)) {
         float top = 0.f;
 #pragma unroll
-        for (int x = tid; x < L::SUBS; x += 256) {
+        for (int x = tid; x < L::SUBS; x += NT) {
             const int tok = t0 * kKeys + 16 * x;
             int block = -1;
             if (x < 4 * nt && tok < live) block = kv8_block(a.c, table, a.max_blocks, tok);
             float ks = 0.f, vs = 0.f;
-            long long off = -1;
+            long long off = 0;
             if (block >= 0) {
                 off = kv8_offset(a.c, block, kvh) + (long long)(tok & ((1 << a.c.bt_log2) - 1)) * D;
                 ks = a.c.k_scales[(long long)block * a.c.n_kv_heads + kvh];
                 vs = a.c.v_scales[(long long)block * a.c.n_kv_heads + kvh];
             }
+            const unsigned long long gone = __ballot(block < 0 && x < 4 * nt && tok < live);
+            if (lane < 2) sub_gone[(x >> 5) + lane] = (uint32_t)(lane ? gone >> 32 : gone);
             sub_off[x] = off;
             sub_ks[x] = ks;
             sub_vs[x] = vs;
@@ -269,46 +320,61 @@ __global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void kv8_prefill_kernel(Kv8Pr
         top = wave_reduce_dpp<true>(top);
         if (lane == 0) misc[wave] = __float_as_int(top);
         __syncthreads();
-        return fmaxf(fmaxf(__int_as_float(misc[0]), __int_as_float(misc[1])),
-                     fmaxf(__int_as_float(misc[2]), __int_as_float(misc[3])));
+        top = 0.f;
+#pragma unroll
+        for (int w = 0; w < WAVES; w++) top = fmaxf(top, __int_as_float(misc[w]));
+        return top;
     };
 
     // ---- staging: codes in registers between their loads and the LDS
     u32x4_t kst[KL];
     uint32_t vst[VL][4];
-    float vsc = 0.f;      // V scale of this thread's tokens
-    bool vdead[4];        // its tokens behind the end
+    float vsc = 0.f;  // V scale of this thread's tokens
     unsigned char* const kslot0 = lds;
     unsigned char* const vslot0 = lds + 2 * L::KBYTES;
-    // K chunk u: token (tid + 256 u) / (D / 16), 16 bytes at (tid % (D / 16))
+    // K chunk u: token (tid + NT u) / (D / 16), 16 bytes at (tid % (D / 16))
     constexpr int CPR = D / 16;
-    // V unit u: four tokens from 4 tg on, four dims from 4 (vc + 8 * u') on
-    const int tg = (lane >> 3) + 8 * (wave & 1);
-    const int vc = (lane & 7) + (D == 128 ? 16 * (wave >> 1) : 8 * (wave >> 1));
-    auto load_tile = [&](int t0, int it) __attribute__((always_inline)) {
-        const int s0 = it * 4;
+    // V unit u: four tokens from 4 tg on, four dims from 4 (vc + 8 u) on.  Of a
+    // wavefront's stores to V^T, 8 bytes a lane, 32 lanes then cover every bank twice.
+    const bool stages_k = !APART || !second, stages_v = !APART || second;
+    const int vwave = APART ? wave & (WAVES / 2 - 1) : wave;
+    const int tg = ((lane >> 2) & 7) + 8 * (vwave & 1);
+    const int vc = (lane & 3) + 4 * (lane >> 5) + 8 * VL * (vwave >> 1);
+    // what the next loads and weights need of the table, read ahead of them
+    long long koff[KL], voff = 0;
+    float vnext = 0.f;
+    float4_t ks4;
+    auto look_k = [&](int it) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < KL; u++) koff[u] = sub_off[4 * it + ((tid + NT * u) / CPR >> 4)];
+    };
+    auto look_v = [&](int it) __attribute__((always_inline)) {
+        voff = sub_off[4 * it + (tg >> 2)];
+        vnext = sub_vs[4 * it + (tg >> 2)];
+    };
+    auto load_k = [&]() __attribute__((always_inline)) {
+        if (!stages_k) return;
 #pragma unroll
         for (int u = 0; u < KL; u++) {
-            const int tk = (tid + 256 * u) / CPR;
-            const long long off = max(sub_off[s0 + (tk >> 4)], 0ll);  // absent: any row, masked
-            kst[u] = *(const u32x4_t*)(a.c.k + off + (tk & 15) * D + 16 * (tid % CPR));
+            const int tk = (tid + NT * u) / CPR;
+            kst[u] = *(const u32x4_t*)(a.c.k + koff[u] + (tk & 15) * D + 16 * (tid % CPR));
         }
-        const long long off = sub_off[s0 + (tg >> 2)];
-        vsc = sub_vs[s0 + (tg >> 2)];
-        const uint8_t* vb = a.c.v + max(off, 0ll) + (tg & 3) * 4 * D + 4 * vc;
+    };
+    auto load_v = [&]() __attribute__((always_inline)) {
+        if (!stages_v) return;
+        vsc = vnext;
+        const uint8_t* vb = a.c.v + voff + (tg & 3) * 4 * D + 4 * vc;
 #pragma unroll
         for (int u = 0; u < VL; u++)
 #pragma unroll
             for (int i = 0; i < 4; i++) vst[u][i] = *(const uint32_t*)(vb + i * D + 32 * u);
-        const int key = (t0 + it) * kKeys + 4 * tg;
-#pragma unroll
-        for (int i = 0; i < 4; i++) vdead[i] = off < 0 || key + i >= live;
     };
-    auto store_tile = [&](int it, float unit) __attribute__((always_inline)) {
+    auto store_k = [&](int it) __attribute__((always_inline)) {
+        if (!stages_k) return;
         unsigned char* ks = kslot0 + (it & 1) * L::KBYTES;
 #pragma unroll
         for (int u = 0; u < KL; u++) {
-            const int tk = (tid + 256 * u) / CPR;
+            const int tk = (tid + NT * u) / CPR;
             u32x4_t y[2];
 #pragma unroll
             for (int e = 0; e < 4; e++) {
@@ -320,6 +386,25 @@ __global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void kv8_prefill_kernel(Kv8Pr
             p[0] = y[0];
             p[1] = y[1];
         }
+    };
+    // bits of a tile's absent subtiles; most tables have none
+    bool any_gone = false;
+    auto gone_of = [&](int it) __attribute__((always_inline)) {
+        return any_gone ? __builtin_amdgcn_readfirstlane((int)((sub_gone[it >> 3] >> (4 * (it & 7))) & 15)) : 0;
+    };
+    auto store_v = [&](int t0, int it, int last, float unit) __attribute__((always_inline)) {
+        if (!stages_v) return;
+        const int key = (t0 + min(it, last)) * kKeys;
+        const int gone = gone_of(min(it, last));
+        if (gone || key + kKeys > live) {
+            asm volatile("");
+            // tokens behind the end and absent ones may hold NaN codes: zeros
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int u = 0; u < VL; u++)
+                    vst[u][i] = ((gone >> (tg >> 2)) & 1) || key + 4 * tg + i >= live ? 0u : vst[u][i];
+        }
         unsigned char* vs = vslot0 + (it & 1) * L::VBYTES;
         const _Float16 f = (_Float16)(vsc * unit);
         const half2_t f2 = {f, f};
@@ -328,7 +413,7 @@ __global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void kv8_prefill_kernel(Kv8Pr
         for (int u = 0; u < VL; u++) {
             uint32_t w[4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) w[i] = kv8_bias<CODE>(vdead[i] ? 0u : vst[u][i]);
+            for (int i = 0; i < 4; i++) w[i] = kv8_bias<CODE>(vst[u][i]);
             uint32_t y[4][2];
 #pragma unroll
             for (int i = 0; i < 2; i++) {
@@ -349,170 +434,310 @@ __global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void kv8_prefill_kernel(Kv8Pr
     };
 
     // ---- one half (32 keys) of a tile
-    auto scores = [&](const unsigned char* ks, int kb, float16_t (&st)[NT]) __attribute__((always_inline)) {
-        const unsigned char* kp = ks + (kb * 32 + j) * L::KROW + 16 * h;
+    auto read_k = [&](int it, int kb, half8_t (&kf)[KS]) __attribute__((always_inline)) {
+        const unsigned char* kp = kslot0 + (it & 1) * L::KBYTES + (32 * kb + j) * L::KROW + 16 * h;
 #pragma unroll
-        for (int t = 0; t < NT; t++) st[t] = float16_t{};
-#pragma unroll
-        for (int s = 0; s < KS; s++) {
-            const half8_t kf = __builtin_bit_cast(half8_t, *(const u32x4_t*)(kp + 32 * s));
-#pragma unroll
-            for (int t = 0; t < NT; t++)
-                st[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qreg[t][s], st[t], 0, 0, 0);
-        }
+        for (int s = 0; s < KS; s++) kf[s] = __builtin_bit_cast(half8_t, *(const u32x4_t*)(kp + 32 * s));
     };
-    auto load_v = [&](const unsigned char* vs, int kb, half8_t (&vf)[2][DT]) __attribute__((always_inline)) {
-        const unsigned char* vp = vs + j * L::VROW + 16 * h + 64 * kb;
+    auto scores = [&](const half8_t (&kf)[KS]) __attribute__((always_inline)) {
+        float16_t st = float16_t{};
 #pragma unroll
-        for (int t2 = 0; t2 < 2; t2++)
+        for (int s = 0; s < KS; s++) st = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[s], qreg[s], st, 0, 0, 0);
+        return st;
+    };
+    auto read_v = [&](int it, int kb, half8_t (&vf)[2][DT]) __attribute__((always_inline)) {
+        const unsigned char* vp = vslot0 + (it & 1) * L::VBYTES + j * L::VROW + 16 * h + 64 * kb;
+#pragma unroll
+        for (int t = 0; t < 2; t++)
 #pragma unroll
             for (int d = 0; d < DT; d++)
-                vf[t2][d] = __builtin_bit_cast(half8_t, *(const u32x4_t*)(vp + 32 * d * L::VROW + 32 * t2));
+                vf[t][d] = __builtin_bit_cast(half8_t, *(const u32x4_t*)(vp + 32 * d * L::VROW + 32 * t));
     };
-    // A lane's score r of half kb is that of key kt + 32 kb + 4 h + 8 (r / 4) + r % 4,
-    // which lies in subtile 2 kb + r / 8.
-    auto consume = [&](float16_t st, const half8_t (&vf)[2][DT], int t, int t0, int it, int kb, bool masked)
-        __attribute__((always_inline)) {
+    auto values = [&](const half8_t (&vf)[2][DT], const half8_t (&pa)[2]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[t][d], pa[t], o[d], 0, 0, 0);
+    };
+    // The weights of a half.  A lane's score r is that of key k0 + c(r), c(r) =
+    // 8 (r / 4) + r % 4, which lies in subtile 2 kb + r / 8.  In log2 units it
+    // is st[r] * f[r / 8] + sb + sl * c(r); `ready` applies what is not linear and
+    // the mask, in branches, so that `weigh` is one block with the products around it.
+    struct Factors {
+        float f[2], sb, sl;
+    };
+    auto ready = [&](float16_t& st, Factors& w, int t0, int it, int kb, bool edge) __attribute__((always_inline)) {
         const int k0 = (t0 + it) * kKeys + 32 * kb + 4 * h;
-        const int s0 = it * 4 + 2 * kb;
-        float f[2];
+        w.sb = w.sl = 0.f;
 #pragma unroll
-        for (int u = 0; u < 2; u++) f[u] = sub_ks[s0 + u] * crow[t];
-        if constexpr (MODS) {
+        for (int u = 0; u < 2; u++) w.f[u] = ks4[2 * kb + u] * crow;
+        if constexpr (CAP) {
+            // cap tanh(x) = cap - 2 cap / (e^2x + 1)
 #pragma unroll
-            for (int r = 0; r < 16; r++) {
-                float x = st[r] * f[r >> 3];
-                if (a.s.cap_log2 > 0.f)  // cap tanh(x), x in natural units
-                    x = __builtin_fmaf(-2.f * a.s.cap_log2,
-                                       __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * 2.885390081777927f) + 1.f),
+            for (int r = 0; r < 16; r++)
+                st[r] = __builtin_fmaf(-2.f * a.s.cap_log2,
+                                       __builtin_amdgcn_rcpf(
+                                           __builtin_amdgcn_exp2f(st[r] * (w.f[r >> 3] * 2.885390081777927f)) + 1.f),
                                        a.s.cap_log2);
-                if (a.s.slopes) x = __builtin_fmaf(-slope[t], fabsf((float)(qpos[t] - k0) - (float)(8 * (r >> 2) + (r & 3))), x);
-                st[r] = x;
-            }
-            f[0] = f[1] = 1.f;
+            w.f[0] = w.f[1] = 1.f;
         }
-        if (masked) {
-            const int lo = key_lo[t] - k0, hi = key_hi[t] - k0;
-            const bool gone[2] = {sub_off[s0] < 0, sub_off[s0 + 1] < 0};
+        if constexpr (BIAS) {
+            w.sl = slope;
+            w.sb = slope * (float)(k0 - qpos);
+            if (a.s.prefix_lens) {  // keys on both sides of the row
+                asm volatile("");
+#pragma unroll
+                for (int r = 0; r < 16; r++)
+                    st[r] = __builtin_fmaf(-slope, fabsf((float)(k0 - qpos) + (float)(8 * (r >> 2) + (r & 3))),
+                                           st[r] * w.f[r >> 3]);
+                w.f[0] = w.f[1] = 1.f;
+                w.sl = w.sb = 0.f;
+            }
+        }
+        if (edge) {
+            asm volatile("");  // a branch: few tiles are
+            const int lo = key_lo - k0, hi = key_hi - k0;
+            const int bits = gone_of(it) >> (2 * kb);
+            const bool gone[2] = {(bits & 1) != 0, (bits & 2) != 0};
 #pragma unroll
             for (int r = 0; r < 16; r++) {
                 const int c = 8 * (r >> 2) + (r & 3);
-                st[r] = c >= lo && c < hi && !gone[r >> 3] ? st[r] * f[r >> 3] : -INFINITY;
+                st[r] = c >= lo && c < hi && !gone[r >> 3] ? st[r] * w.f[r >> 3] : -INFINITY;
             }
-            f[0] = f[1] = 1.f;
+            w.f[0] = w.f[1] = 1.f;
         }
-        half8_t pa[2];
+    };
+    // N halves against one maximum: it may move only while no weights wait for
+    // their product.
+    auto weigh = [&](auto n, const float16_t* st, const Factors* w, half8_t (*pa)[2]) __attribute__((always_inline)) {
+        constexpr int N = decltype(n)::value;
         float psum;
         auto exps = [&]() __attribute__((always_inline)) {
-            float sa = 0.f, sb = 0.f;
+            float sa = 0.f, sc = 0.f;
 #pragma unroll
-            for (int r = 0; r < 16; r += 2) {
-                const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(st[r], f[r >> 3], -mrun[t]));
-                const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(st[r + 1], f[r >> 3], -mrun[t]));
-                sa += p0;
-                sb += p1;
-                pa[r >> 3][r & 7] = (_Float16)p0;
-                pa[r >> 3][(r & 7) + 1] = (_Float16)p1;
+            for (int kb = 0; kb < N; kb++) {
+                const float base = w[kb].sb - mrun;
+#pragma unroll
+                for (int r = 0; r < 16; r += 2) {
+                    const int c = 8 * (r >> 2) + (r & 3);
+                    const float b0 = BIAS ? __builtin_fmaf(w[kb].sl, (float)c, base) : base;
+                    const float b1 = BIAS ? __builtin_fmaf(w[kb].sl, (float)(c + 1), base) : base;
+                    const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(st[kb][r], w[kb].f[r >> 3], b0));
+                    const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(st[kb][r + 1], w[kb].f[r >> 3], b1));
+                    sa += p0;
+                    sc += p1;
+                    pa[kb][r >> 3][r & 7] = (_Float16)p0;
+                    pa[kb][r >> 3][(r & 7) + 1] = (_Float16)p1;
+                }
             }
-            psum = sa + sb;
+            psum = sa + sc;
         };
         exps();
         if (__any(psum > kSumLimit)) {
             float top = -INFINITY;
 #pragma unroll
-            for (int r = 0; r < 16; r++) top = fmaxf(top, st[r] * f[r >> 3]);
-            const float mnew = fmaxf(mrun[t], max_half(top));
-            const float down = __builtin_amdgcn_exp2f(mrun[t] - mnew);
-            mrun[t] = mnew;
-            lrun[t] *= down;
+            for (int kb = 0; kb < N; kb++)
 #pragma unroll
-            for (int d = 0; d < DT; d++) o[t][d] *= down;
+                for (int r = 0; r < 16; r++) {
+                    const float bias =
+                        BIAS ? __builtin_fmaf(w[kb].sl, (float)(8 * (r >> 2) + (r & 3)), w[kb].sb) : 0.f;
+                    top = fmaxf(top, __builtin_fmaf(st[kb][r], w[kb].f[r >> 3], bias));
+                }
+            // only this pair's own sum moves it: a pair's result is its own, whatever
+            // pairs share the wavefront
+            const float mnew = max_half(psum) > kSumLimit ? fmaxf(mrun, max_half(top)) : mrun;
+            const float down = __builtin_amdgcn_exp2f(mrun - mnew);
+            mrun = mnew;
+            lrun *= down;
+#pragma unroll
+            for (int d = 0; d < DT; d++) o[d] *= down;
             exps();
         }
-        lrun[t] += psum;
-#pragma unroll
-        for (int t2 = 0; t2 < 2; t2++)
-#pragma unroll
-            for (int d = 0; d < DT; d++)
-                o[t][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[t2][d], pa[t2], o[t][d], 0, 0, 0);
+        lrun += psum;
     };
 
     float unit = 0.f;  // the largest V scale so far: what O is measured in
     for (int base = 0; base < n_tiles; base += kTableTiles) {
         const int t0 = t_first + base;
         const int nt = min(kTableTiles, n_tiles - base);
-        if (base) __syncthreads();  // the table is still read
+        if (base) __syncthreads();  // the table and the tiles are still read
         const float top = fmaxf(fill(t0, nt), kVLeast);
         if (top > unit) {
             const float down = unit / top;
 #pragma unroll
-            for (int t = 0; t < NT; t++)
-#pragma unroll
-                for (int d = 0; d < DT; d++) o[t][d] *= down;
+            for (int d = 0; d < DT; d++) o[d] *= down;
             unit = top;
         }
-        // At the top of step `it` the LDS slots it & 1 hold tile it, and the
-        // registers tile it + 1, whose loads were issued a step earlier.
-        load_tile(t0, 0);
-        store_tile(0, kVUnit / unit);
-        if (nt > 1) load_tile(t0, 1);
-        __syncthreads();
-        for (int it = 0; it < nt; it++) {
-            if (it + 1 < nt) store_tile(it + 1, kVUnit / unit);
-            if (it + 2 < nt) load_tile(t0, it + 2);
-            const unsigned char* ks = kslot0 + (it & 1) * L::KBYTES;
-            const unsigned char* vs = vslot0 + (it & 1) * L::VBYTES;
+        const float vunit = kVUnit / unit;
+        any_gone = __any(lane < L::SUBS / 32 && sub_gone[lane & (L::SUBS / 32 - 1)] != 0);
+        // whether a tile has keys that some row of the wavefront does not see
+        auto at_edge = [&](int it) {
             const int kt = (t0 + it) * kKeys;
-            const bool gone = (sub_off[4 * it] | sub_off[4 * it + 1] | sub_off[4 * it + 2] | sub_off[4 * it + 3]) < 0;
-            const bool masked = gone || kt + kKeys > w_hi || kt < w_lo;
-            float16_t st0[NT], st1[NT];
-            half8_t vf[2][DT];
-            scores(ks, 0, st0);
-            load_v(vs, 0, vf);
-            scores(ks, 1, st1);
-#pragma unroll
-            for (int t = 0; t < NT; t++) consume(st0[t], vf, t, t0, it, 0, masked);
-            load_v(vs, 1, vf);
-#pragma unroll
-            for (int t = 0; t < NT; t++) consume(st1[t], vf, t, t0, it, 1, masked);
+            return gone_of(it) || kt + kKeys > w_hi || kt < w_lo;
+        };
+        const int last = nt - 1;
+        constexpr std::integral_constant<int, 1> one{};
+        constexpr std::integral_constant<int, 2> two{};
+        if constexpr (PHASES) {
+            // Before the phases: K of tile 0, and the second half's part of K of
+            // tile 1 and V of tile 0 (the first half's follow in its first phase).
+            const int ahead = second ? 1 : 0;
+            look_k(0);
+            load_k();
+            store_k(0);
+            look_k(min(1, last));
+            look_v(0);
+            load_k();
+            load_v();
+            if (second) {
+                store_k(1);
+                store_v(t0, 0, last, vunit);
+                look_k(min(2, last));
+                look_v(min(1, last));
+                load_k();
+                load_v();
+            }
             __syncthreads();
+            float16_t st[2];
+            {
+                half8_t kf[KS];
+                read_k(0, 0, kf);
+                st[0] = scores(kf);
+                read_k(0, 1, kf);
+                st[1] = scores(kf);
+            }
+            ks4 = *(const float4_t*)sub_ks;
+            look_k(min(ahead + 2, last));
+            look_v(min(ahead + 1, last));
+            if (second) __syncthreads();
+            for (int it = 0; it < nt; it++) {
+                half8_t pa[2][2];
+                {
+                    const bool edge = at_edge(it);
+                    Factors w[2];
+                    ready(st[0], w[0], t0, it, 0, edge);
+                    ready(st[1], w[1], t0, it, 1, edge);
+                    weigh(two, st, w, pa);
+                    store_k(it + ahead + 1);
+                    store_v(t0, it + ahead, last, vunit);
+                    load_k();
+                    load_v();
+                }
+                __syncthreads();
+                __builtin_amdgcn_s_setprio(1);
+                {
+                    half8_t kf[2][KS], vf[2][2][DT];
+                    st[0] = st[1] = float16_t{};
+                    read_k(it + 1, 0, kf[0]);
+                    read_k(it + 1, 1, kf[1]);
+#pragma unroll
+                    for (int s = 0; s < KS; s++)
+#pragma unroll
+                        for (int kb = 0; kb < 2; kb++)
+                            st[kb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[kb][s], qreg[s], st[kb], 0, 0, 0);
+                    read_v(it, 0, vf[0]);
+                    read_v(it, 1, vf[1]);
+                    values(vf[0], pa[0]);
+                    values(vf[1], pa[1]);
+                    ks4 = *(const float4_t*)(sub_ks + 4 * min(it + 1, last));
+                    look_k(min(it + ahead + 3, last));
+                    look_v(min(it + ahead + 2, last));
+                    // reads run AHEAD products in front: an LDS round trip is four of them
+                    constexpr int READS = 2 * KS + 4 * DT, AHEAD = 10;
+                    __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
+#pragma unroll
+                    for (int i = 0; i < READS - AHEAD; i++) {
+                        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                    }
+                    __builtin_amdgcn_sched_group_barrier(0x8, AHEAD, 0);
+                }
+                __builtin_amdgcn_s_setprio(0);
+                __syncthreads();
+            }
+            if (!second) __syncthreads();
+        } else {
+            // One barrier a step, behind the last use of its K: in front of it K and
+            // V slots it & 1 hold tile it and K slot it + 1 & 1 is complete behind it;
+            // the step writes K of tile it + 2 and V of tile it + 1 from registers and
+            // requests the next (past the last tile it repeats that one, into slots
+            // that nobody reads).  Operands are read well ahead of their products.
+            look_k(0);
+            look_v(0);
+            load_k();
+            load_v();
+            store_k(0);
+            store_v(t0, 0, last, vunit);
+            look_k(min(1, last));
+            look_v(min(1, last));
+            load_k();
+            load_v();
+            store_k(1);
+            look_k(min(2, last));
+            load_k();
+            __syncthreads();
+            half8_t kf[KS], vf[2][DT];
+            read_k(0, 0, kf);
+            float16_t st0 = scores(kf);
+            for (int it = 0; it < nt; it++) {
+                const bool edge = at_edge(it);
+                half8_t pa[2][2];
+                Factors w;
+                ks4 = *(const float4_t*)(sub_ks + 4 * it);
+                read_k(it, 1, kf);
+                __builtin_amdgcn_sched_barrier(0);
+                ready(st0, w, t0, it, 0, edge);
+                float16_t st1 = scores(kf);
+                weigh(one, &st0, &w, pa);
+                __syncthreads();
+                read_v(it, 0, vf);
+                look_v(min(it + 2, last));
+                look_k(min(it + 3, last));
+                __builtin_amdgcn_sched_barrier(0);
+                ready(st1, w, t0, it, 1, edge);
+                values(vf, pa[0]);  // ahead of the next weights, which may move the maximum
+                read_k(it + 1, 0, kf);
+                weigh(one, &st1, &w, pa + 1);
+                store_v(t0, it + 1, last, vunit);
+                store_k(it + 2);
+                load_v();
+                load_k();
+                read_v(it, 1, vf);
+                __builtin_amdgcn_sched_barrier(0);
+                st0 = scores(kf);
+                values(vf, pa[1]);
+            }
         }
     }
 
     // ---- results
-    float l[NT], m[NT];
+    float l = sum_half(lrun), m = mrun;
 #pragma unroll
-    for (int t = 0; t < NT; t++) {
-        l[t] = sum_half(lrun[t]);
-        m[t] = mrun[t];
-#pragma unroll
-        for (int d = 0; d < DT; d++) o[t][d] *= unit / kVUnit;
-    }
+    for (int d = 0; d < DT; d++) o[d] *= unit / kVUnit;
     if (n_pieces > 1) {
-        // [piece][wavefront][pair tile][dim tile][4 registers][lane]
-        const long long slot0 = item * a.pieces;
+        // [piece][wavefront][dim tile][4 registers][lane]
+        const long long slot0 = (long long)item * a.pieces;
+        const bool holds = tile * TM + wave * kWavePairs < pairs;  // pairs of the wavefront
         constexpr int PART = TM * D;
         const auto acc_at = [&](int p) {
-            return partial_rsrc(a.ws_o + (slot0 + p) * PART + wave * (PART / 4), PART);
+            return partial_rsrc(a.ws_o + (slot0 + p) * PART + wave * (PART / WAVES), PART / WAVES * 4);
         };
         const auto ml_at = [&](int p) {
-            return partial_rsrc(a.ws_ml + ((slot0 + p) * 4 + wave) * NT * 64, NT * 64 * 8);
+            return partial_rsrc(a.ws_ml + ((slot0 + p) * WAVES + wave) * 64, 64 * 8);
         };
-        {
+        if (holds) {
             const __amdgpu_buffer_rsrc_t ro = acc_at(piece), rm = ml_at(piece);
 #pragma unroll
-            for (int t = 0; t < NT; t++) {
+            for (int d = 0; d < DT; d++)
 #pragma unroll
-                for (int d = 0; d < DT; d++)
-#pragma unroll
-                    for (int r = 0; r < 4; r++)
-                        __builtin_amdgcn_raw_buffer_store_b128(
-                            u32x4_t{__float_as_uint(o[t][d][4 * r]), __float_as_uint(o[t][d][4 * r + 1]),
-                                    __float_as_uint(o[t][d][4 * r + 2]), __float_as_uint(o[t][d][4 * r + 3])},
-                            ro, (((t * DT + d) * 4 + r) * 64 + lane) * 16, 0, kSc1);
-                __builtin_amdgcn_raw_buffer_store_b64(u32x2_t{__float_as_uint(m[t]), __float_as_uint(l[t])}, rm,
-                                                      (t * 64 + lane) * 8, 0, kSc1);
-            }
+                for (int r = 0; r < 4; r++)
+                    __builtin_amdgcn_raw_buffer_store_b128(
+                            u32x4_t{__float_as_uint(o[d][4 * r]), __float_as_uint(o[d][4 * r + 1]),
+                                    __float_as_uint(o[d][4 * r + 2]), __float_as_uint(o[d][4 * r + 3])},
+                            ro, ((d * 4 + r) * 64 + lane) * 16, 0, kSc1);
+                __builtin_amdgcn_raw_buffer_store_b64(u32x2_t{__float_as_uint(m), __float_as_uint(l)}, rm, lane * 8, 0,
+                                                  kSc1);
         }
         // every wavefront's stores have completed before the arrival is counted
         __atomic_signal_fence(__ATOMIC_SEQ_CST);
@@ -522,45 +747,53 @@ __global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void kv8_prefill_kernel(Kv8Pr
             misc[8] = __hip_atomic_fetch_add(a.counters + item, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         __syncthreads();
         if (misc[8] != n_pieces - 1) return;
+        m = -1e30f;
+        l = 0.f;
 #pragma unroll
-        for (int t = 0; t < NT; t++) {
-            m[t] = -1e30f;
-            l[t] = 0.f;
-#pragma unroll
-            for (int d = 0; d < DT; d++) o[t][d] = float16_t{};
-        }
-        for (int p = 0; p < n_pieces; p++) {
+        for (int d = 0; d < DT; d++) o[d] = float16_t{};
+        // a piece's loads are on their way while the one before is joined
+        struct Part {
+            u32x2_t ml;
+            u32x4_t w[DT][4];
+        } x, y;
+        const auto fetch = [&](Part& q, int p) __attribute__((always_inline)) {
             const __amdgpu_buffer_rsrc_t ro = acc_at(p), rm = ml_at(p);
+            q.ml = __builtin_amdgcn_raw_buffer_load_b64(rm, lane * 8, 0, kSc1);
 #pragma unroll
-            for (int t = 0; t < NT; t++) {
-                const u32x2_t ml = __builtin_amdgcn_raw_buffer_load_b64(rm, (t * 64 + lane) * 8, 0, kSc1);
-                u32x4_t w[DT][4];
+            for (int d = 0; d < DT; d++)
 #pragma unroll
-                for (int d = 0; d < DT; d++)
+                for (int r = 0; r < 4; r++)
+                    q.w[d][r] = __builtin_amdgcn_raw_buffer_load_b128(ro, ((d * 4 + r) * 64 + lane) * 16, 0, kSc1);
+        };
+        const auto join = [&](const Part& q) __attribute__((always_inline)) {
+            const float mp = __uint_as_float(q.ml[0]);
+            const float mnew = fmaxf(m, mp);
+            const float f0 = __builtin_amdgcn_exp2f(m - mnew), f1 = __builtin_amdgcn_exp2f(mp - mnew);
+            m = mnew;
+            l = __builtin_fmaf(__uint_as_float(q.ml[1]), f1, l * f0);
 #pragma unroll
-                    for (int r = 0; r < 4; r++)
-                        w[d][r] = __builtin_amdgcn_raw_buffer_load_b128(
-                            ro, (((t * DT + d) * 4 + r) * 64 + lane) * 16, 0, kSc1);
-                const float mp = __uint_as_float(ml[0]);
-                const float mnew = fmaxf(m[t], mp);
-                const float f0 = __builtin_amdgcn_exp2f(m[t] - mnew), f1 = __builtin_amdgcn_exp2f(mp - mnew);
-                m[t] = mnew;
-                l[t] = __builtin_fmaf(__uint_as_float(ml[1]), f1, l[t] * f0);
+            for (int d = 0; d < DT; d++)
 #pragma unroll
-                for (int d = 0; d < DT; d++)
-#pragma unroll
-                    for (int r = 0; r < 16; r++)
-                        o[t][d][r] = __builtin_fmaf(__uint_as_float(w[d][r >> 2][r & 3]), f1, o[t][d][r] * f0);
+                for (int r = 0; r < 16; r++)
+                    o[d][r] = __builtin_fmaf(__uint_as_float(q.w[d][r >> 2][r & 3]), f1, o[d][r] * f0);
+        };
+        if (holds) {
+            fetch(x, 0);
+            for (int p = 0; p < n_pieces; p += 2) {
+                if (p + 1 < n_pieces) fetch(y, p + 1);
+                join(x);
+                if (p + 1 >= n_pieces) break;
+                if (p + 2 < n_pieces) fetch(x, p + 2);
+                join(y);
             }
         }
         if (tid == 0) __hip_atomic_store(a.counters + item, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
-#pragma unroll
-    for (int t = 0; t < NT; t++) {
-        const int x = tile * TM + (wave * NT + t) * 32 + j;
-        if (x >= pairs) continue;
+    {
+        const int x = tile * TM + wave * kWavePairs + j;
+        if (x >= pairs) return;
         const int i = x / a.group;
-        const float inv = l[t] == 0.f ? 0.f : 1.f / l[t];  // nothing seen: zeros
+        const float inv = l == 0.f ? 0.f : 1.f / l;  // nothing seen: zeros
         uint16_t* orow = a.out + ((long long)(row0 + i) * a.n_heads + kvh * a.group + (x - i * a.group)) * D + 4 * h;
 #pragma unroll
         for (int d = 0; d < DT; d++)
@@ -568,19 +801,17 @@ __global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void kv8_prefill_kernel(Kv8Pr
             for (int r = 0; r < 4; r++) {
                 typedef __bf16 bf16x4_t __attribute__((ext_vector_type(4)));
                 *(bf16x4_t*)(orow + 32 * d + 8 * r) =
-                    bf16x4_t{(__bf16)(o[t][d][4 * r] * inv), (__bf16)(o[t][d][4 * r + 1] * inv),
-                             (__bf16)(o[t][d][4 * r + 2] * inv), (__bf16)(o[t][d][4 * r + 3] * inv)};
+                    bf16x4_t{(__bf16)(o[d][4 * r] * inv), (__bf16)(o[d][4 * r + 1] * inv),
+                             (__bf16)(o[d][4 * r + 2] * inv), (__bf16)(o[d][4 * r + 3] * inv)};
             }
     }
 }
 
 // ------------------------------------------------------------- host side
 
-constexpr int kPieceTiles = 4;   // fewest tiles of a piece
-constexpr int kMaxPieces = 16;
 
 struct Kv8PrefillPlan {
-    int chunk, nt, pieces;
+    int chunk, waves, pieces;
     long long items;  // (tile, kv head)s of a launch at most
     size_t o, ml, bytes;
 };
@@ -597,20 +828,35 @@ static int prefill_plan(Kv8PrefillPlan& p, const Kv8& c, int batch, int n_heads,
         return set_error(NYION_ERR_UNSUPPORTED, "%s: n_rows %d * n_heads %d beyond 2^27", what, n_rows, n_heads);
     const int group = n_heads / c.n_kv_heads;
     p.chunk = std::min(batch, kSeqsMax);
-    p.nt = 1;
-    const int tm = 128 * p.nt;
-    // tiles: one partial tile per sequence at most, besides the whole ones
-    p.items = ((long long)n_rows * group / tm + std::min(p.chunk, n_rows)) * c.n_kv_heads;
+    // tiles of a launch at most: the whole ones, and a partial one per sequence
+    const auto items = [&](int waves) {
+        return ((long long)n_rows * group / (kWavePairs * waves) + std::min(p.chunk, n_rows)) * c.n_kv_heads;
+    };
+    const long long cus = device_cu_count();
+    // Eight wavefronts in two phases at head_dim 128 where they give every CU two
+    // workgroups or more in turn, four without phases elsewhere.  Measured (us, four /
+    // eight; 32/8 heads of 128): 8192 rows (1024 workgroups of eight) 615 / 552, 4096
+    // (512) 176 / 149, four sequences of 1500 behind 500 (768) 185 / 167, 3000 (375) 108 /
+    // 127, 2048 (256) 61 / 76; 32/4 heads of 64, whose products are too short to hide the
+    // other phase, 8192 rows 443 / 537.
+    p.waves = c.head_dim == 128 && items(8) >= 2 * cus ? 8 : 4;
+    const int tm = kWavePairs * p.waves;
+    p.items = items(p.waves);
     if (p.items >= (1 << 24)) return set_error(NYION_ERR_UNSUPPORTED, "%s: %lld tiles", what, p.items);
     const long long keys = window > 0 ? std::min((long long)window + max_rows, (long long)max_ctx) : max_ctx;
     const long long tiles = (keys + kKeys - 1) / kKeys;
-    const long long fill = p.items > 0 ? 4LL * device_cu_count() / p.items : 1;
+    // Keys are cut only where all pieces are resident at once: a piece's partial result
+    // is 64 KB at head_dim 128, written and read again past L2.  (Cutting the long tiles
+    // of launches that fill the chip, to even out the causal triangle, measured 158 us
+    // against 105 for 3000 rows of 32/8 heads of 128.)
+    const long long resident = cus * (p.waves == 8 ? 1 : c.head_dim == 128 ? 2 : 3);
+    const long long fill = p.items > 0 ? resident / p.items : 1;
     p.pieces = (int)std::max(1LL, std::min({fill, tiles / kPieceTiles, (long long)kMaxPieces}));
     p.o = p.ml = p.bytes = 0;
     if (p.pieces > 1) {
         const size_t slots = (size_t)p.items * p.pieces;
         p.o = slots * tm * c.head_dim * sizeof(float);
-        p.ml = slots * 4 * p.nt * 64 * sizeof(float2);
+        p.ml = slots * p.waves * 64 * sizeof(float2);
         p.bytes = p.o + p.ml + (((size_t)p.items * sizeof(int) + 255) & ~(size_t)255);
     }
     return NYION_OK;
@@ -677,9 +923,7 @@ int nyion_kv8_prefill_attention_bf16(const nyion_kv8_cache* cache, const int32_t
     a.n_heads = n_heads;
     a.group = n_heads / a.c.n_kv_heads;
     a.pieces = p.pieces;
-    a.min_tiles = kPieceTiles;
     a.max_items = (int)p.items;
-    const bool mods = a.s.cap_log2 > 0.f || a.s.slopes;
     const int grid = (int)((p.items * p.pieces + 7) / 8 * 8);
     const int32_t* prefix = a.s.prefix_lens;
     for (int b0 = 0; b0 < batch; b0 += p.chunk) {
@@ -688,22 +932,31 @@ int nyion_kv8_prefill_attention_bf16(const nyion_kv8_cache* cache, const int32_t
         a.ctx_lens = ctx_lens + b0;
         a.row_starts = row_starts + b0;
         a.s.prefix_lens = prefix ? prefix + b0 : nullptr;
-        auto launch = [&](auto d, auto code, auto m) {
+        auto launch = [&](auto d, auto code, auto cap, auto bias) {
             constexpr int D = decltype(d)::value, CODE = decltype(code)::value;
-            constexpr bool MODS = decltype(m)::value;
-            hipLaunchKernelGGL((kv8_prefill_kernel<D, CODE, MODS, 1>), dim3(grid), dim3(256), 0, (hipStream_t)stream, a);
-        };
-        auto by_mods = [&](auto d, auto code) {
-            if (mods)
-                launch(d, code, std::true_type{});
+            constexpr bool CAP = decltype(cap)::value, BIAS = decltype(bias)::value;
+            if (p.waves == 8)
+                hipLaunchKernelGGL((kv8_prefill_kernel<D, CODE, CAP, BIAS, 8>), dim3(grid), dim3(512), 0,
+                                   (hipStream_t)stream, a);
             else
-                launch(d, code, std::false_type{});
+                hipLaunchKernelGGL((kv8_prefill_kernel<D, CODE, CAP, BIAS, 4>), dim3(grid), dim3(256), 0,
+                                   (hipStream_t)stream, a);
+        };
+        auto by_options = [&](auto d, auto code) {
+            if (a.s.cap_log2 > 0.f && a.s.slopes)
+                launch(d, code, std::true_type{}, std::true_type{});
+            else if (a.s.cap_log2 > 0.f)
+                launch(d, code, std::true_type{}, std::false_type{});
+            else if (a.s.slopes)
+                launch(d, code, std::false_type{}, std::true_type{});
+            else
+                launch(d, code, std::false_type{}, std::false_type{});
         };
         auto by_code = [&](auto d) {
             if (cache->code == NYION_KV8_E4M3)
-                by_mods(d, std::integral_constant<int, NYION_KV8_E4M3>{});
+                by_options(d, std::integral_constant<int, NYION_KV8_E4M3>{});
             else
-                by_mods(d, std::integral_constant<int, NYION_KV8_INT8>{});
+                by_options(d, std::integral_constant<int, NYION_KV8_INT8>{});
         };
         if (a.c.head_dim == 64)
             by_code(std::integral_constant<int, 64>{});
