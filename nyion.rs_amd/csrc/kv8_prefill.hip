@@ -344,13 +344,13 @@ __global__ __launch_bounds__(64 * WAVES, 2 * 4 / WAVES) void kv8_prefill_kernel(
     long long koff[KL], voff = 0;
     float vnext = 0.f;
     float4_t ks4;
-    auto look_k = [&](int it) __attribute__((always_inline)) {
+    auto look_k = [&](int x) __attribute__((always_inline)) {
 #pragma unroll
-        for (int u = 0; u < KL; u++) koff[u] = sub_off[4 * it + ((tid + NT * u) / CPR >> 4)];
+        for (int u = 0; u < KL; u++) koff[u] = sub_off[4 * x + ((tid + NT * u) / CPR >> 4)];
     };
-    auto look_v = [&](int it) __attribute__((always_inline)) {
-        voff = sub_off[4 * it + (tg >> 2)];
-        vnext = sub_vs[4 * it + (tg >> 2)];
+    auto look_v = [&](int x) __attribute__((always_inline)) {
+        voff = sub_off[4 * x + (tg >> 2)];
+        vnext = sub_vs[4 * x + (tg >> 2)];
     };
     auto load_k = [&]() __attribute__((always_inline)) {
         if (!stages_k) return;
@@ -389,13 +389,13 @@ __global__ __launch_bounds__(64 * WAVES, 2 * 4 / WAVES) void kv8_prefill_kernel(
     };
     // bits of a tile's absent subtiles; most tables have none
     bool any_gone = false;
-    auto gone_of = [&](int it) __attribute__((always_inline)) {
-        return any_gone ? __builtin_amdgcn_readfirstlane((int)((sub_gone[it >> 3] >> (4 * (it & 7))) & 15)) : 0;
+    auto gone_of = [&](int x) __attribute__((always_inline)) {
+        return any_gone ? __builtin_amdgcn_readfirstlane((int)((sub_gone[x >> 3] >> (4 * (x & 7))) & 15)) : 0;
     };
-    auto store_v = [&](int t0, int it, int last, float unit) __attribute__((always_inline)) {
+    auto store_v = [&](int t0, int it, int x, float unit) __attribute__((always_inline)) {
         if (!stages_v) return;
-        const int key = (t0 + min(it, last)) * kKeys;
-        const int gone = gone_of(min(it, last));
+        const int key = (t0 + x) * kKeys;
+        const int gone = gone_of(x);
         if (gone || key + kKeys > live) {
             asm volatile("");
             // tokens behind the end and absent ones may hold NaN codes: zeros
@@ -467,8 +467,8 @@ __global__ __launch_bounds__(64 * WAVES, 2 * 4 / WAVES) void kv8_prefill_kernel(
     struct Factors {
         float f[2], sb, sl;
     };
-    auto ready = [&](float16_t& st, Factors& w, int t0, int it, int kb, bool edge) __attribute__((always_inline)) {
-        const int k0 = (t0 + it) * kKeys + 32 * kb + 4 * h;
+    auto ready = [&](float16_t& st, Factors& w, int t0, int x, int kb, bool edge) __attribute__((always_inline)) {
+        const int k0 = (t0 + x) * kKeys + 32 * kb + 4 * h;
         w.sb = w.sl = 0.f;
 #pragma unroll
         for (int u = 0; u < 2; u++) w.f[u] = ks4[2 * kb + u] * crow;
@@ -498,7 +498,7 @@ __global__ __launch_bounds__(64 * WAVES, 2 * 4 / WAVES) void kv8_prefill_kernel(
         if (edge) {
             asm volatile("");  // a branch: few tiles are
             const int lo = key_lo - k0, hi = key_hi - k0;
-            const int bits = gone_of(it) >> (2 * kb);
+            const int bits = gone_of(x) >> (2 * kb);
             const bool gone[2] = {(bits & 1) != 0, (bits & 2) != 0};
 #pragma unroll
             for (int r = 0; r < 16; r++) {
@@ -558,10 +558,13 @@ __global__ __launch_bounds__(64 * WAVES, 2 * 4 / WAVES) void kv8_prefill_kernel(
     };
 
     float unit = 0.f;  // the largest V scale so far: what O is measured in
-    for (int base = 0; base < n_tiles; base += kTableTiles) {
+    // From the last keys to the first: those next to a row have its largest scores
+    // where they are biased by distance, and its maximum then hardly moves (8192 rows
+    // with slopes of 2^-8 to 2^-1/4: 870 -> 557 us).
+    for (int base = (n_tiles - 1) / kTableTiles * kTableTiles; base >= 0 && n_tiles > 0; base -= kTableTiles) {
         const int t0 = t_first + base;
         const int nt = min(kTableTiles, n_tiles - base);
-        if (base) __syncthreads();  // the table and the tiles are still read
+        if (unit > 0.f) __syncthreads();  // the table and the tiles are still read
         const float top = fmaxf(fill(t0, nt), kVLeast);
         if (top > unit) {
             const float down = unit / top;
@@ -572,29 +575,31 @@ __global__ __launch_bounds__(64 * WAVES, 2 * 4 / WAVES) void kv8_prefill_kernel(
         const float vunit = kVUnit / unit;
         any_gone = __any(lane < L::SUBS / 32 && sub_gone[lane & (L::SUBS / 32 - 1)] != 0);
         // whether a tile has keys that some row of the wavefront does not see
-        auto at_edge = [&](int it) {
-            const int kt = (t0 + it) * kKeys;
-            return gone_of(it) || kt + kKeys > w_hi || kt < w_lo;
-        };
         const int last = nt - 1;
+        // the table's tile of a step, the last one's past the end
+        const auto tile_of = [&](int it) { return max(last - it, 0); };
+        auto at_edge = [&](int it) {
+            const int kt = (t0 + tile_of(it)) * kKeys;
+            return gone_of(tile_of(it)) || kt + kKeys > w_hi || kt < w_lo;
+        };
         constexpr std::integral_constant<int, 1> one{};
         constexpr std::integral_constant<int, 2> two{};
         if constexpr (PHASES) {
             // Before the phases: K of tile 0, and the second half's part of K of
             // tile 1 and V of tile 0 (the first half's follow in its first phase).
             const int ahead = second ? 1 : 0;
-            look_k(0);
+            look_k(last);
             load_k();
             store_k(0);
-            look_k(min(1, last));
-            look_v(0);
+            look_k(tile_of(1));
+            look_v(last);
             load_k();
             load_v();
             if (second) {
                 store_k(1);
-                store_v(t0, 0, last, vunit);
-                look_k(min(2, last));
-                look_v(min(1, last));
+                store_v(t0, 0, tile_of(0), vunit);
+                look_k(tile_of(2));
+                look_v(tile_of(1));
                 load_k();
                 load_v();
             }
@@ -607,20 +612,20 @@ __global__ __launch_bounds__(64 * WAVES, 2 * 4 / WAVES) void kv8_prefill_kernel(
                 read_k(0, 1, kf);
                 st[1] = scores(kf);
             }
-            ks4 = *(const float4_t*)sub_ks;
-            look_k(min(ahead + 2, last));
-            look_v(min(ahead + 1, last));
+            ks4 = *(const float4_t*)(sub_ks + 4 * last);
+            look_k(tile_of(ahead + 2));
+            look_v(tile_of(ahead + 1));
             if (second) __syncthreads();
             for (int it = 0; it < nt; it++) {
                 half8_t pa[2][2];
                 {
                     const bool edge = at_edge(it);
                     Factors w[2];
-                    ready(st[0], w[0], t0, it, 0, edge);
-                    ready(st[1], w[1], t0, it, 1, edge);
+                    ready(st[0], w[0], t0, tile_of(it), 0, edge);
+                    ready(st[1], w[1], t0, tile_of(it), 1, edge);
                     weigh(two, st, w, pa);
                     store_k(it + ahead + 1);
-                    store_v(t0, it + ahead, last, vunit);
+                    store_v(t0, it + ahead, tile_of(it + ahead), vunit);
                     load_k();
                     load_v();
                 }
@@ -640,9 +645,9 @@ __global__ __launch_bounds__(64 * WAVES, 2 * 4 / WAVES) void kv8_prefill_kernel(
                     read_v(it, 1, vf[1]);
                     values(vf[0], pa[0]);
                     values(vf[1], pa[1]);
-                    ks4 = *(const float4_t*)(sub_ks + 4 * min(it + 1, last));
-                    look_k(min(it + ahead + 3, last));
-                    look_v(min(it + ahead + 2, last));
+                    ks4 = *(const float4_t*)(sub_ks + 4 * tile_of(it + 1));
+                    look_k(tile_of(it + ahead + 3));
+                    look_v(tile_of(it + ahead + 2));
                     // reads run AHEAD products in front: an LDS round trip is four of them
                     constexpr int READS = 2 * KS + 4 * DT, AHEAD = 10;
                     __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
@@ -663,18 +668,18 @@ __global__ __launch_bounds__(64 * WAVES, 2 * 4 / WAVES) void kv8_prefill_kernel(
             // the step writes K of tile it + 2 and V of tile it + 1 from registers and
             // requests the next (past the last tile it repeats that one, into slots
             // that nobody reads).  Operands are read well ahead of their products.
-            look_k(0);
-            look_v(0);
+            look_k(last);
+            look_v(last);
             load_k();
             load_v();
             store_k(0);
-            store_v(t0, 0, last, vunit);
-            look_k(min(1, last));
-            look_v(min(1, last));
+            store_v(t0, 0, tile_of(0), vunit);
+            look_k(tile_of(1));
+            look_v(tile_of(1));
             load_k();
             load_v();
             store_k(1);
-            look_k(min(2, last));
+            look_k(tile_of(2));
             load_k();
             __syncthreads();
             half8_t kf[KS], vf[2][DT];
@@ -684,22 +689,22 @@ __global__ __launch_bounds__(64 * WAVES, 2 * 4 / WAVES) void kv8_prefill_kernel(
                 const bool edge = at_edge(it);
                 half8_t pa[2][2];
                 Factors w;
-                ks4 = *(const float4_t*)(sub_ks + 4 * it);
+                ks4 = *(const float4_t*)(sub_ks + 4 * tile_of(it));
                 read_k(it, 1, kf);
                 __builtin_amdgcn_sched_barrier(0);
-                ready(st0, w, t0, it, 0, edge);
+                ready(st0, w, t0, tile_of(it), 0, edge);
                 float16_t st1 = scores(kf);
                 weigh(one, &st0, &w, pa);
                 __syncthreads();
                 read_v(it, 0, vf);
-                look_v(min(it + 2, last));
-                look_k(min(it + 3, last));
+                look_v(tile_of(it + 2));
+                look_k(tile_of(it + 3));
                 __builtin_amdgcn_sched_barrier(0);
-                ready(st1, w, t0, it, 1, edge);
+                ready(st1, w, t0, tile_of(it), 1, edge);
                 values(vf, pa[0]);  // ahead of the next weights, which may move the maximum
                 read_k(it + 1, 0, kf);
                 weigh(one, &st1, &w, pa + 1);
-                store_v(t0, it + 1, last, vunit);
+                store_v(t0, it + 1, tile_of(it + 1), vunit);
                 store_k(it + 2);
                 load_v();
                 load_k();
