@@ -134,9 +134,8 @@ struct Kv8Span {
     int first;       // tile of lo
     int tiles;       // at least 1: an empty range has a tile with every key masked
 };
-__device__ __forceinline__ Kv8Span kv8_span(const Kv8DecodeArgs& a, int b) {
+__device__ __forceinline__ Kv8Span kv8_span(const Kv8DecodeArgs& a, int ctx) {
     Kv8Span r;
-    const int ctx = a.ctx_lens[b];
     r.hi = max(min(ctx, a.span), 0);
     r.lo = a.s.window > 0 && ctx > a.s.window ? ctx - a.s.window : 0;
     if (r.lo > r.hi) r.lo = r.hi;
@@ -146,7 +145,7 @@ __device__ __forceinline__ Kv8Span kv8_span(const Kv8DecodeArgs& a, int b) {
 }
 
 template <int D, int CODE, bool MODS>
-__global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void kv8_decode_kernel(Kv8DecodeArgs a) {
+__global__ __launch_bounds__(64 * kWaves, 2) void kv8_decode_kernel(Kv8DecodeArgs a) {
     using Tile = Kv8Tile<D>;
     constexpr int KC = Tile::KC, VW = Tile::VW;
     constexpr int MT = D / 16;       // 16-dim tiles of O^T
@@ -155,7 +154,10 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void kv8_decode_kerne
     __shared__ float2 sm_ml[kWaves][16];
     __shared__ int sm_ends[kMaxSeqs];
     __shared__ int sm_wave[kWaves];
-    __shared__ int sm_last;
+    __shared__ struct {
+        int seg, n_pieces, slot0, slot1, b, head0, heads;
+    } sm_shared[2];
+    __shared__ int sm_last[2];
 
     const int tid = threadIdx.x;
     const int lane = tid & 63;
@@ -167,11 +169,12 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void kv8_decode_kerne
     // Where this workgroup's tiles lie: of `total` tiles each of `wgs`
     // workgroups takes total / wgs, the first total % wgs one more.
     uint32_t pos = 0, end = 0, wgs = 0, share = 0, extra = 0;
-    int seq_end = 0;  // up to 64 sequences: lane b holds the tiles up to and with b
+    int seq_ctx = 0, seq_end = 0;  // up to 64 sequences: lane b holds b's length, and the tiles up to and with b
     if (a.pieces == 0) {
         uint32_t total;
         if (a.batch <= 64) {
-            seq_end = lane < a.batch ? kv8_span(a, lane).tiles : 0;
+            seq_ctx = lane < a.batch ? a.ctx_lens[lane] : 0;
+            seq_end = lane < a.batch ? kv8_span(a, seq_ctx).tiles : 0;
 #pragma unroll
             for (int d = 1; d < 64; d <<= 1) {
                 const int y = __shfl_up(seq_end, d);
@@ -182,7 +185,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void kv8_decode_kerne
             int before = 0;
             for (int b0 = 0; b0 < a.batch; b0 += 64 * kWaves) {
                 const int b = b0 + tid;
-                int x = b < a.batch ? kv8_span(a, b).tiles : 0;
+                int x = b < a.batch ? kv8_span(a, a.ctx_lens[b]).tiles : 0;
 #pragma unroll
                 for (int d = 1; d < 64; d <<= 1) {
                     const int y = __shfl_up(x, d);
@@ -217,32 +220,60 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void kv8_decode_kerne
     };
     const auto first_tile = [&](uint32_t w) { return share * w + min(w, extra); };
 
+    // results: a thread holds DPT dims of a head
+    constexpr int DPT = D / 16;
+    const int row = tid >> 4;
+    const int d0 = (tid & 15) * DPT;
+    const auto write_out = [&](const float (&o)[DPT], float ol, int b, int head0, int heads) __attribute__((always_inline)) {
+        if (row >= heads) return;
+        const float inv = ol == 0.f ? 0.f : 1.f / ol;  // nothing seen: zeros
+        const long long at = ((long long)b * a.n_heads + head0 + row) * D + d0;
+        if (a.bf16) {
+#pragma unroll
+            for (int e = 0; e < DPT; e += 4) {
+                typedef __bf16 bf16x4_t __attribute__((ext_vector_type(4)));
+                *(bf16x4_t*)((uint16_t*)a.out + at + e) =
+                    bf16x4_t{(__bf16)(o[e] * inv), (__bf16)(o[e + 1] * inv), (__bf16)(o[e + 2] * inv),
+                             (__bf16)(o[e + 3] * inv)};
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < DPT; e += 4)
+                *(float4_t*)((float*)a.out + at + e) =
+                    float4_t{o[e] * inv, o[e + 1] * inv, o[e + 2] * inv, o[e + 3] * inv};
+        }
+    };
+    const __amdgpu_buffer_rsrc_t racc = partial_rsrc(a.ws_acc, (uint32_t)a.slots * 16 * D * 4);
+    const __amdgpu_buffer_rsrc_t rml = partial_rsrc(a.ws_ml, (uint32_t)a.slots * 16 * 8);
+    int n_shared = 0;  // segments that other workgroups have pieces of
+    const int slot_step = a.pieces > 0 ? 1 : 2;
+
     while (true) {
         int seg, t0, t1, n_pieces;
-        long long slot_mine, slot0, slot1;  // partials: piece 0's, and piece p >= 1's less stride (p - 1)
-        int slot_step;
+        int slot_mine, slot0, slot1;  // partials: piece 0's, and piece p >= 1's less slot_step (p - 1)
         Kv8Span sp;
-        int b;
+        int b, ctx;
         if (a.pieces > 0) {
             seg = (int)blockIdx.x / a.pieces;
             const int p = (int)blockIdx.x - seg * a.pieces;
             b = seg / units;
-            sp = kv8_span(a, b);
+            ctx = __builtin_amdgcn_readfirstlane(a.ctx_lens[b]);
+            sp = kv8_span(a, ctx);
             n_pieces = min(a.pieces, (sp.tiles + a.min_tiles - 1) / a.min_tiles);
             if (p >= n_pieces) return;
             // pieces of tiles / n_pieces, the first ones one more
             const int part = sp.tiles / n_pieces, more = sp.tiles - part * n_pieces;
             t0 = part * p + min(p, more);
             t1 = t0 + part + (p < more ? 1 : 0);
-            slot0 = (long long)seg * a.pieces;
+            slot0 = seg * a.pieces;
             slot1 = slot0 + 1;
-            slot_step = 1;
             slot_mine = slot0 + p;
         } else {
             int before;  // tiles of the sequences in front
             if (a.batch <= 64) {
                 b = (int)__builtin_ctzll(__ballot((uint32_t)seq_end * units > pos));
                 before = b > 0 ? __builtin_amdgcn_readlane(seq_end, b - 1) : 0;
+                ctx = __builtin_amdgcn_readlane(seq_ctx, b);
             } else {
                 int lo = 0, hi = a.batch - 1;  // first sequence whose tiles end behind pos
                 while (lo < hi) {
@@ -254,8 +285,9 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void kv8_decode_kerne
                 }
                 b = __builtin_amdgcn_readfirstlane(lo);
                 before = b > 0 ? __builtin_amdgcn_readfirstlane(sm_ends[b - 1]) : 0;
+                ctx = __builtin_amdgcn_readfirstlane(a.ctx_lens[b]);
             }
-            sp = kv8_span(a, b);
+            sp = kv8_span(a, ctx);
             const uint32_t seq0 = (uint32_t)before * units;
             const uint32_t unit = (pos - seq0) / (uint32_t)sp.tiles;
             const uint32_t start = seq0 + unit * sp.tiles;  // of the segment
@@ -268,11 +300,10 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void kv8_decode_kerne
             } else {
                 const uint32_t w0 = holder(start), w1 = holder(start + sp.tiles - 1);
                 n_pieces = (int)(w1 - w0) + 1;
-                slot0 = 2 * (long long)w0 + (first_tile(w0) >= start ? 0 : 1);
-                slot1 = 2 * (long long)(w0 + 1);
-                slot_mine = 2 * (long long)blockIdx.x + (first_segment ? 0 : 1);
+                slot0 = 2 * (int)w0 + (first_tile(w0) >= start ? 0 : 1);
+                slot1 = 2 * (int)(w0 + 1);
+                slot_mine = 2 * (int)blockIdx.x + (first_segment ? 0 : 1);
             }
-            slot_step = 2;
         }
         const int unit = seg - b * units;
         const int kvh = unit / a.n_hg;
@@ -280,7 +311,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void kv8_decode_kerne
         const int head0 = kvh * a.group + hg * 16;
         const int heads = min(16, a.group - hg * 16);
         const int32_t* table = a.tables + (long long)b * a.max_blocks;
-        const int qpos = a.ctx_lens[b] - 1;
+        const int qpos = ctx - 1;
 
         float slope = 0.f;
         if (MODS && a.s.slopes && n < heads) slope = a.s.slopes[head0 + n] * 1.4426950408889634f;
@@ -293,21 +324,23 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void kv8_decode_kerne
 
         // this wavefront's tiles
         const int tn = t1 - t0;
-        int tw = sp.first + t0 + tn * wave / kWaves;
-        const int tw1 = sp.first + t0 + tn * (wave + 1) / kWaves;
+        const int tw0 = sp.first + t0 + tn * wave / kWaves;
+        int te = sp.first + t0 + tn * (wave + 1) / kWaves;
 
         const uint32_t klane = (uint32_t)((4 * (n & 3) + (n >> 2)) * D + 16 * g);
         const uint32_t vlane = (uint32_t)(g * D + 4 * VW * n);
 
-        // up to 16 tiles, 64 subtiles, from tile t on: a lane looks up one
-        // subtile's place and scales
+        // the last 16 tiles, 64 subtiles, in front of tile te, from tb on: a lane looks
+        // up one subtile's place and scales
         long long off = 0;
         float ks = 0.f, vs = 0.f;
         unsigned long long absent = 0;
-        auto look_up = [&](int t) __attribute__((always_inline)) {
-            const int tok = t * kTile + 16 * lane;
+        int tb = 0;
+        auto look_up = [&]() __attribute__((always_inline)) {
+            tb = max(tw0, te - 16);
+            const int tok = tb * kTile + 16 * lane;
             int block = -1;
-            if (lane < 4 * (tw1 - t) && tok < sp.hi && tok + 16 > sp.lo) block = kv8_block(a.c, table, a.max_blocks, tok);
+            if (lane < 4 * (te - tb) && tok < sp.hi && tok + 16 > sp.lo) block = kv8_block(a.c, table, a.max_blocks, tok);
             const bool present = block >= 0;
             off = 0;
             ks = vs = 0.f;
@@ -341,8 +374,8 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void kv8_decode_kerne
             }
         };
         // the first tile's rows are on their way while q is split
-        Tile ta, tb;
-        if (tw < tw1) look_up(tw);
+        Tile tile_a, tile_b;
+        if (tw0 < te) look_up();
         // q of head n as two binary16 terms of q * 2^-e, largest in [2^13, 2^14)
         half8_t qh[2 * KC], ql[2 * KC];
         float crow;  // what a score is multiplied with, besides the K scale
@@ -367,7 +400,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void kv8_decode_kerne
                 for (int e = 0; e < 4; e++) xq[c][e] = u[e], xq[c][4 + e] = v[e];
             }
         }
-        if (tw < tw1) load(ta, 0);
+        if (tw0 < te) load(tile_a, te - tb - 1);
         {
             float top = 0.f;
 #pragma unroll
@@ -389,8 +422,9 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void kv8_decode_kerne
             crow = __builtin_amdgcn_ldexpf(a.s.scale_log2, ex);
         }
 
-        while (tw < tw1) {
-            const int nt = min(16, tw1 - tw);
+        // from the last tile to the first: scores biased by distance then leave the
+        // maximum alone
+        while (tw0 < te) {
             // the weights' unit: the largest V scale
             {
                 const float top = fmaxf(wave_reduce_dpp<true>(fabsf(vs)), kLeastScale);
@@ -404,29 +438,31 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void kv8_decode_kerne
             const float cvl = vs / unit_scale * kWeightUnit;
 
             auto use = [&](Tile& t, int i) __attribute__((always_inline)) {
-                const int p0 = (tw + i) * kTile;
+                const int p0 = (tb + i) * kTile;
                 const int gone = (int)(absent >> (4 * i)) & 15;
                 const bool masked = p0 < sp.lo || p0 > sp.hi - kTile || gone;
-                // the four subtiles' chains side by side: a chain's MFMAs wait for each other
+                // two subtiles' chains side by side: a chain's MFMAs wait for each other
                 float4_t s[4];
 #pragma unroll
                 for (int u = 0; u < 4; u++) s[u] = float4_t{};
 #pragma unroll
-                for (int c = 0; c < 2 * KC; c++) {
-                    half8_t kh[4];
+                for (int u0 = 0; u0 < 4; u0 += 2)
 #pragma unroll
-                    for (int u = 0; u < 4; u++) {
-                        const uint32_t w0 = kv8_bias<CODE>(t.k[u][c >> 1][2 * (c & 1)]);
-                        const uint32_t w1 = kv8_bias<CODE>(t.k[u][c >> 1][2 * (c & 1) + 1]);
-                        const u32x4_t kf = {kv8_pair<CODE, false>(w0), kv8_pair<CODE, true>(w0),
-                                            kv8_pair<CODE, false>(w1), kv8_pair<CODE, true>(w1)};
-                        kh[u] = __builtin_bit_cast(half8_t, kf);
-                        s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh[u], qh[c], s[u], 0, 0, 0);
+                    for (int c = 0; c < 2 * KC; c++) {
+                        half8_t kh[2];
+#pragma unroll
+                        for (int u = 0; u < 2; u++) {
+                            const uint32_t w0 = kv8_bias<CODE>(t.k[u0 + u][c >> 1][2 * (c & 1)]);
+                            const uint32_t w1 = kv8_bias<CODE>(t.k[u0 + u][c >> 1][2 * (c & 1) + 1]);
+                            const u32x4_t kf = {kv8_pair<CODE, false>(w0), kv8_pair<CODE, true>(w0),
+                                                kv8_pair<CODE, false>(w1), kv8_pair<CODE, true>(w1)};
+                            kh[u] = __builtin_bit_cast(half8_t, kf);
+                            s[u0 + u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh[u], qh[c], s[u0 + u], 0, 0, 0);
+                        }
+#pragma unroll
+                        for (int u = 0; u < 2; u++)
+                            s[u0 + u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh[u], ql[c], s[u0 + u], 0, 0, 0);
                     }
-#pragma unroll
-                    for (int u = 0; u < 4; u++)
-                        s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh[u], ql[c], s[u], 0, 0, 0);
-                }
                 // log2 scores are s * f
                 float f[4];
 #pragma unroll
@@ -541,18 +577,18 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void kv8_decode_kerne
                         }
                     }
             };
-            int i = 0;
-            for (; i + 1 < nt; i += 2) {
-                load(tb, i + 1);
-                use(ta, i);
-                load(ta, min(i + 2, nt - 1));
-                use(tb, i + 1);
+            int i = te - tb - 1;
+            for (; i > 0; i -= 2) {
+                load(tile_b, i - 1);
+                use(tile_a, i);
+                load(tile_a, max(i - 2, 0));
+                use(tile_b, i - 1);
             }
-            if (i < nt) use(ta, i);
-            tw += nt;
-            if (tw < tw1) {
-                look_up(tw);
-                load(ta, 0);
+            if (i == 0) use(tile_a, 0);
+            te = tb;
+            if (tw0 < te) {
+                look_up();
+                load(tile_a, te - tb - 1);
             }
         }
 
@@ -569,9 +605,6 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void kv8_decode_kerne
             if (g == 0) sm_ml[wave][n] = float2{m, l};
         }
         __syncthreads();
-        constexpr int DPT = D / 16;  // dims per thread
-        const int row = tid >> 4;
-        const int d0 = (tid & 15) * DPT;
         float o[DPT];
         float om = -INFINITY, ol = 0.f;
 #pragma unroll
@@ -587,32 +620,11 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void kv8_decode_kerne
 #pragma unroll
             for (int e = 0; e < DPT; e++) o[e] = __builtin_fmaf(sm_acc[w][row][d0 + e], f, o[e]);
         }
-        auto write_out = [&]() {
-            if (row >= heads) return;
-            const float inv = ol == 0.f ? 0.f : 1.f / ol;  // nothing seen: zeros
-            const long long at = ((long long)b * a.n_heads + head0 + row) * D + d0;
-            if (a.bf16) {
-#pragma unroll
-                for (int e = 0; e < DPT; e += 4) {
-                    typedef __bf16 bf16x4_t __attribute__((ext_vector_type(4)));
-                    *(bf16x4_t*)((uint16_t*)a.out + at + e) =
-                        bf16x4_t{(__bf16)(o[e] * inv), (__bf16)(o[e + 1] * inv), (__bf16)(o[e + 2] * inv),
-                                 (__bf16)(o[e + 3] * inv)};
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < DPT; e += 4)
-                    *(float4_t*)((float*)a.out + at + e) =
-                        float4_t{o[e] * inv, o[e + 1] * inv, o[e + 2] * inv, o[e + 3] * inv};
-            }
-        };
         if (n_pieces == 1) {
-            write_out();
+            write_out(o, ol, b, head0, heads);
         } else {
-            const __amdgpu_buffer_rsrc_t racc = partial_rsrc(a.ws_acc, (uint32_t)a.slots * 16 * D * 4);
-            const __amdgpu_buffer_rsrc_t rml = partial_rsrc(a.ws_ml, (uint32_t)a.slots * 16 * 8);
             if (row < heads) {
-                const int mine = (int)slot_mine * 16 + row;
+                const int mine = slot_mine * 16 + row;
 #pragma unroll
                 for (int e = 0; e < DPT; e += 4)
                     __builtin_amdgcn_raw_buffer_store_b128(
@@ -623,91 +635,105 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void kv8_decode_kerne
                     __builtin_amdgcn_raw_buffer_store_b64(u32x2_t{__float_as_uint(om), __float_as_uint(ol)}, rml,
                                                           mine * 8, 0, kSc1);
             }
-            // every wavefront's stores have completed before the arrival is counted
-            __atomic_signal_fence(__ATOMIC_SEQ_CST);
-            __builtin_amdgcn_s_waitcnt(0);
-            __syncthreads();
-            if (tid == 0)
-                sm_last = __hip_atomic_fetch_add(a.counters + seg, 1, __ATOMIC_RELAXED,
-                                                 __HIP_MEMORY_SCOPE_AGENT) == n_pieces - 1;
-            __syncthreads();
-            if (sm_last) {
-                // 16 threads a head; what is left of the workgroup takes every
-                // `groups`-th piece, so that one round of loads has many
-                const int rows = heads > 8 ? 16 : heads > 4 ? 8 : heads > 2 ? 4 : heads;  // a power of two
-                const int groups = 16 / rows;
-                const int mrow = row & (rows - 1), mgrp = row / rows;
-                const int rr = min(mrow, heads - 1);  // rows behind the last hold nothing
-                om = -INFINITY;
-                ol = 0.f;
-#pragma unroll
-                for (int e = 0; e < DPT; e++) o[e] = 0.f;
-                constexpr int AHEAD = 8;
-                for (int p = mgrp; p < n_pieces; p += AHEAD * groups) {
-                    u32x4_t w[AHEAD][DPT / 4];
-                    u32x2_t ml[AHEAD];
-#pragma unroll
-                    for (int k = 0; k < AHEAD; k++) {
-                        const int pk = min(p + k * groups, n_pieces - 1);
-                        const int slot = (int)(pk == 0 ? slot0 : slot1 + slot_step * (pk - 1));
-                        // slots are at most 2 * kMaxWgs: their bytes stay in 32 bits
-                        ml[k] = __builtin_amdgcn_raw_buffer_load_b64(rml, (slot * 16 + rr) * 8, 0, kSc1);
-#pragma unroll
-                        for (int e = 0; e < DPT / 4; e++)
-                            w[k][e] = __builtin_amdgcn_raw_buffer_load_b128(
-                                racc, ((slot * 16 + rr) * D + d0 + 4 * e) * 4, 0, kSc1);
-                    }
-                    float top = om;
-#pragma unroll
-                    for (int k = 0; k < AHEAD; k++) top = fmaxf(top, __uint_as_float(ml[k][0]));
-                    const float base = top == -INFINITY ? 0.f : top;
-                    const float down = __builtin_amdgcn_exp2f(om - base);
-                    om = top;
-                    ol *= down;
-#pragma unroll
-                    for (int e = 0; e < DPT; e++) o[e] *= down;
-#pragma unroll
-                    for (int k = 0; k < AHEAD; k++) {
-                        if (p + k * groups >= n_pieces) break;
-                        const float f = __builtin_amdgcn_exp2f(__uint_as_float(ml[k][0]) - base);
-                        ol = __builtin_fmaf(__uint_as_float(ml[k][1]), f, ol);
-#pragma unroll
-                        for (int e = 0; e < DPT; e++)
-                            o[e] = __builtin_fmaf(__uint_as_float(w[k][e >> 2][e & 3]), f, o[e]);
-                    }
-                }
-                if (groups > 1) {
-                    float* const part = &sm_acc[0][0][0];  // [groups * rows = 16][D + PAD]
-#pragma unroll
-                    for (int e = 0; e < DPT; e++) part[row * (D + PAD) + d0 + e] = o[e];
-                    if ((tid & 15) == 0) sm_ml[0][row] = float2{om, ol};
-                    __syncthreads();
-                    om = -INFINITY;
-                    ol = 0.f;
-#pragma unroll
-                    for (int e = 0; e < DPT; e++) o[e] = 0.f;
-                    if (row < rows) {
-                        for (int k = 0; k < groups; k++) om = fmaxf(om, sm_ml[0][k * rows + row].x);
-                        const float base = om == -INFINITY ? 0.f : om;
-                        for (int k = 0; k < groups; k++) {
-                            const float2 ml = sm_ml[0][k * rows + row];
-                            const float f = __builtin_amdgcn_exp2f(ml.x - base);
-                            ol = __builtin_fmaf(ml.y, f, ol);
-#pragma unroll
-                            for (int e = 0; e < DPT; e++)
-                                o[e] = __builtin_fmaf(part[(k * rows + row) * (D + PAD) + d0 + e], f, o[e]);
-                        }
-                    }
-                }
-                write_out();
-                if (tid == 0) __hip_atomic_store(a.counters + seg, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            }
+            if (tid == 0) sm_shared[n_shared] = {seg, n_pieces, slot0, slot1, b, head0, heads};
+            n_shared++;
         }
-        if (a.pieces > 0) return;
+        if (a.pieces > 0) break;
         pos += t1 - t0;
         first_segment = false;
-        if (pos >= end) return;
+        if (pos >= end) break;
         __syncthreads();  // LDS is free for the next segment
+    }
+    if (n_shared == 0) return;
+
+    // At most two segments of a workgroup are shared, its first and its last.
+    // Their arrivals are counted here, in one round trip: every wavefront's stores
+    // have completed before (the first's long ago).
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (tid < n_shared) {
+        sm_last[tid] = __hip_atomic_fetch_add(a.counters + sm_shared[tid].seg, 1, __ATOMIC_RELAXED,
+                                              __HIP_MEMORY_SCOPE_AGENT) == sm_shared[tid].n_pieces - 1;
+    }
+    __syncthreads();
+    const bool last0 = __builtin_amdgcn_readfirstlane(sm_last[0]) != 0;
+    const bool last1 = n_shared > 1 && __builtin_amdgcn_readfirstlane(sm_last[1]) != 0;
+#pragma unroll 1
+    for (int k = 0; k < 2; k++) {
+        if (!(k ? last1 : last0)) continue;
+        if (k && last0) __syncthreads();  // LDS still holds the other's parts
+        const auto sh = sm_shared[k];
+        const int heads = sh.heads, n_pieces = sh.n_pieces;
+        // 16 threads a head; what is left of the workgroup takes every
+        // `groups`-th piece, so that one round of loads has many
+        const int rows = heads > 8 ? 16 : heads > 4 ? 8 : heads > 2 ? 4 : heads;  // a power of two
+        const int groups = 16 / rows;
+        const int mrow = row & (rows - 1), mgrp = row / rows;
+        const int rr = min(mrow, heads - 1);  // rows behind the last hold nothing
+        float o[DPT];
+        float om = -INFINITY, ol = 0.f;
+#pragma unroll
+        for (int e = 0; e < DPT; e++) o[e] = 0.f;
+        constexpr int AHEAD = 8;
+        for (int p = mgrp; p < n_pieces; p += AHEAD * groups) {
+            u32x4_t w[AHEAD][DPT / 4];
+            u32x2_t ml[AHEAD];
+#pragma unroll
+            for (int k = 0; k < AHEAD; k++) {
+                const int pk = min(p + k * groups, n_pieces - 1);
+                const int slot = pk == 0 ? sh.slot0 : sh.slot1 + slot_step * (pk - 1);
+                // slots are at most 2 * kMaxWgs: their bytes stay in 32 bits
+                ml[k] = __builtin_amdgcn_raw_buffer_load_b64(rml, (slot * 16 + rr) * 8, 0, kSc1);
+#pragma unroll
+                for (int e = 0; e < DPT / 4; e++)
+                    w[k][e] = __builtin_amdgcn_raw_buffer_load_b128(
+                        racc, ((slot * 16 + rr) * D + d0 + 4 * e) * 4, 0, kSc1);
+            }
+            float top = om;
+#pragma unroll
+            for (int k = 0; k < AHEAD; k++) top = fmaxf(top, __uint_as_float(ml[k][0]));
+            const float base = top == -INFINITY ? 0.f : top;
+            const float down = __builtin_amdgcn_exp2f(om - base);
+            om = top;
+            ol *= down;
+#pragma unroll
+            for (int e = 0; e < DPT; e++) o[e] *= down;
+#pragma unroll
+            for (int k = 0; k < AHEAD; k++) {
+                if (p + k * groups >= n_pieces) break;
+                const float f = __builtin_amdgcn_exp2f(__uint_as_float(ml[k][0]) - base);
+                ol = __builtin_fmaf(__uint_as_float(ml[k][1]), f, ol);
+#pragma unroll
+                for (int e = 0; e < DPT; e++)
+                    o[e] = __builtin_fmaf(__uint_as_float(w[k][e >> 2][e & 3]), f, o[e]);
+            }
+        }
+        if (groups > 1) {
+            float* const part = &sm_acc[0][0][0];  // [groups * rows = 16][D + PAD]
+#pragma unroll
+            for (int e = 0; e < DPT; e++) part[row * (D + PAD) + d0 + e] = o[e];
+            if ((tid & 15) == 0) sm_ml[0][row] = float2{om, ol};
+            __syncthreads();
+            om = -INFINITY;
+            ol = 0.f;
+#pragma unroll
+            for (int e = 0; e < DPT; e++) o[e] = 0.f;
+            if (row < rows) {
+                for (int k = 0; k < groups; k++) om = fmaxf(om, sm_ml[0][k * rows + row].x);
+                const float base = om == -INFINITY ? 0.f : om;
+                for (int k = 0; k < groups; k++) {
+                    const float2 ml = sm_ml[0][k * rows + row];
+                    const float f = __builtin_amdgcn_exp2f(ml.x - base);
+                    ol = __builtin_fmaf(ml.y, f, ol);
+#pragma unroll
+                    for (int e = 0; e < DPT; e++)
+                        o[e] = __builtin_fmaf(part[(k * rows + row) * (D + PAD) + d0 + e], f, o[e]);
+                }
+            }
+        }
+        write_out(o, ol, sh.b, sh.head0, heads);
+        if (tid == 0) __hip_atomic_store(a.counters + sh.seg, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
 }
 
