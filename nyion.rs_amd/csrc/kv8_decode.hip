@@ -739,10 +739,15 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_decode_kernel(Kv8DecodeArg
 
 // ------------------------------------------------------------- host side
 
-// Tiles per workgroup at least, one per wavefront; a launch of at most
-// kDirectSegments segments cuts each of them by itself.
+// Tiles per workgroup at least, one per wavefront.
 constexpr int kMinTiles = 4;
+// A launch of at most this many segments cuts each of them by itself, into as
+// many pieces as give one workgroup per CU, 32 at most: the join reads them
+// all.  Measured (us, two workgroups per CU / one / one and 32 pieces at most):
+// one sequence of 32768 tokens, 32/4 heads of 64, 32.2 / 20.4 / 16.0, 32/8 of 128
+// 25.4 / 21.1 / 21.1; three of 3000-9000, 32/8 of 128, 18.2 / 17.1 / 17.2.
 constexpr int kDirectSegments = 64;
+constexpr long long kMaxDirectPieces = 32;
 
 struct Kv8DecodePlan {
     int units, chunk, pieces, grid;
@@ -765,7 +770,7 @@ static int decode_plan(Kv8DecodePlan& p, const Kv8& c, int batch, int n_heads, i
     const long long keys = window > 0 ? std::min((long long)window + kTile, (long long)max_ctx) : max_ctx;
     const long long tiles = (keys + kTile - 1) / kTile;
     if (segments <= kDirectSegments) {
-        const long long fill = std::max(2 * device_cu_count() / segments, 1LL);
+        const long long fill = std::min(std::max(device_cu_count() / segments, 1LL), kMaxDirectPieces);
         p.pieces = (int)std::min(fill, (tiles + kMinTiles - 1) / kMinTiles);
         p.grid = (int)(segments * p.pieces);
     } else {
