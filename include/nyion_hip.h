@@ -696,8 +696,10 @@ int nyion_kv8_write(const nyion_kv8_cache* cache, const int64_t* slots, int n_ro
  * that head's row of out NaN.
  * d_workspace: nyion_kv8_decode_workspace_size bytes, 256-byte aligned,
  * zero-filled before its first use (nyion_decode_workspace_init) and left with
- * its counters at zero by every call; calls that may overlap in time, replays
- * of captured graphs among them, need workspaces of their own. */
+ * its counters, the first 16 KB, at zero by every call.  One workspace, as
+ * large as the largest needs, serves calls of any shapes of this entry and of
+ * nyion_kv8_prefill_attention_bf16, one after the other; calls that may overlap
+ * in time, replays of captured graphs among them, need workspaces of their own. */
 size_t nyion_kv8_decode_workspace_size(const nyion_kv8_cache* cache, int batch, int n_heads,
                                        int max_ctx, int window);
 int nyion_kv8_decode_attention(const nyion_kv8_cache* cache, const int32_t* block_tables,

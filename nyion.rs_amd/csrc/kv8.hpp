@@ -29,6 +29,11 @@ struct ScoreArgs {
     const int32_t* prefix_lens;
 };
 
+// Workspaces of both attentions begin with their arrival counters, in a place
+// that no argument moves: one workspace then serves calls of any shapes.
+constexpr int kKv8Counters = 4096;
+constexpr size_t kKv8CounterBytes = kKv8Counters * sizeof(int);
+
 // Host: checks a caller's cache struct and fills `c`.
 int kv8_cache_args(Kv8& c, const nyion_kv8_cache* cache, const char* what);
 // Host: checks a caller's options (nullptr: none) and fills `s`.

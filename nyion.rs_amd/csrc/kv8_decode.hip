@@ -49,7 +49,7 @@ namespace nyion {
 
 constexpr int kTile = 64;            // tokens
 constexpr int kMaxSeqs = 1024;       // sequences per launch
-constexpr int kMaxWgs = 2048;        // workgroups per launch (sizes the workspace)
+constexpr int kMaxWgs = kKv8Counters / 2;  // workgroups per launch, two partials each
 constexpr int kWaves = 4;
 constexpr float kWeightUnit = 16384.f;
 constexpr float kLeastScale = 7.888609052210118e-31f;  // 2^-100
@@ -64,7 +64,7 @@ struct Kv8DecodeArgs {
     long long q_stride;
     float* ws_acc;   // [slots][16][D]
     float2* ws_ml;   // [slots][16]
-    int* counters;   // [segments]
+    int* counters;   // [kKv8Counters], by the slot of a segment's first piece
     int max_blocks;
     int span;        // tokens that a table covers
     int batch;
@@ -155,7 +155,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_decode_kernel(Kv8DecodeArg
     __shared__ int sm_ends[kMaxSeqs];
     __shared__ int sm_wave[kWaves];
     __shared__ struct {
-        int seg, n_pieces, slot0, slot1, b, head0, heads;
+        int n_pieces, slot0, slot1, b, head0, heads;
     } sm_shared[2];
     __shared__ int sm_last[2];
 
@@ -635,7 +635,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_decode_kernel(Kv8DecodeArg
                     __builtin_amdgcn_raw_buffer_store_b64(u32x2_t{__float_as_uint(om), __float_as_uint(ol)}, rml,
                                                           mine * 8, 0, kSc1);
             }
-            if (tid == 0) sm_shared[n_shared] = {seg, n_pieces, slot0, slot1, b, head0, heads};
+            if (tid == 0) sm_shared[n_shared] = {n_pieces, slot0, slot1, b, head0, heads};
             n_shared++;
         }
         if (a.pieces > 0) break;
@@ -653,7 +653,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_decode_kernel(Kv8DecodeArg
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
     if (tid < n_shared) {
-        sm_last[tid] = __hip_atomic_fetch_add(a.counters + sm_shared[tid].seg, 1, __ATOMIC_RELAXED,
+        sm_last[tid] = __hip_atomic_fetch_add(a.counters + sm_shared[tid].slot0, 1, __ATOMIC_RELAXED,
                                               __HIP_MEMORY_SCOPE_AGENT) == sm_shared[tid].n_pieces - 1;
     }
     __syncthreads();
@@ -733,7 +733,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_decode_kernel(Kv8DecodeArg
             }
         }
         write_out(o, ol, sh.b, sh.head0, heads);
-        if (tid == 0) __hip_atomic_store(a.counters + sh.seg, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (tid == 0) __hip_atomic_store(a.counters + sh.slot0, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
 }
 
@@ -781,8 +781,7 @@ static int decode_plan(Kv8DecodePlan& p, const Kv8& c, int batch, int n_heads, i
     const size_t slots = (size_t)p.slots;
     p.acc = slots * 16 * c.head_dim * sizeof(float);
     p.ml = (slots * 16 * sizeof(float2) + 255) & ~(size_t)255;
-    p.bytes = p.acc + p.ml + (((size_t)segments * sizeof(int) + 255) & ~(size_t)255);
-    if (p.pieces == 1) p.bytes = 0;
+    p.bytes = p.pieces == 1 ? 0 : kKv8CounterBytes + p.acc + p.ml;
     return NYION_OK;
 }
 
@@ -856,9 +855,9 @@ int nyion_kv8_decode_attention(const nyion_kv8_cache* cache, const int32_t* bloc
         if (!aligned(d_workspace, 256))
             return set_error(NYION_ERR_INVALID, "%s: workspace not 256-byte aligned", what);
     }
-    a.ws_acc = (float*)d_workspace;
-    a.ws_ml = (float2*)((char*)d_workspace + p.acc);
-    a.counters = (int*)((char*)d_workspace + p.acc + p.ml);
+    a.counters = (int*)d_workspace;
+    a.ws_acc = (float*)((char*)d_workspace + kKv8CounterBytes);
+    a.ws_ml = (float2*)((char*)a.ws_acc + p.acc);
     a.q_stride = q_stride;
     a.max_blocks = max_blocks_per_seq;
     a.span = (int)std::min((long long)max_blocks_per_seq << a.c.bt_log2, (long long)INT_MAX - 2 * kTile);

@@ -855,14 +855,14 @@ static int prefill_plan(Kv8PrefillPlan& p, const Kv8& c, int batch, int n_heads,
     // of launches that fill the chip, to even out the causal triangle, measured 158 us
     // against 105 for 3000 rows of 32/8 heads of 128.)
     const long long resident = cus * (p.waves == 8 ? 1 : c.head_dim == 128 ? 2 : 3);
-    const long long fill = p.items > 0 ? resident / p.items : 1;
+    const long long fill = p.items > 0 && p.items <= kKv8Counters ? resident / p.items : 1;
     p.pieces = (int)std::max(1LL, std::min({fill, tiles / kPieceTiles, (long long)kMaxPieces}));
     p.o = p.ml = p.bytes = 0;
     if (p.pieces > 1) {
         const size_t slots = (size_t)p.items * p.pieces;
         p.o = slots * tm * c.head_dim * sizeof(float);
         p.ml = slots * p.waves * 64 * sizeof(float2);
-        p.bytes = p.o + p.ml + (((size_t)p.items * sizeof(int) + 255) & ~(size_t)255);
+        p.bytes = kKv8CounterBytes + p.o + p.ml;
     }
     return NYION_OK;
 }
@@ -916,9 +916,9 @@ int nyion_kv8_prefill_attention_bf16(const nyion_kv8_cache* cache, const int32_t
         if (!aligned(d_workspace, 256))
             return set_error(NYION_ERR_INVALID, "%s: workspace not 256-byte aligned", what);
     }
-    a.ws_o = (float*)d_workspace;
-    a.ws_ml = (float2*)((char*)d_workspace + p.o);
-    a.counters = (int*)((char*)d_workspace + p.o + p.ml);
+    a.counters = (int*)d_workspace;
+    a.ws_o = (float*)((char*)d_workspace + kKv8CounterBytes);
+    a.ws_ml = (float2*)((char*)a.ws_o + p.o);
     a.q = q;
     a.out = out;
     a.q_stride = q_stride;

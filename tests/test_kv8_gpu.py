@@ -281,7 +281,7 @@ def unit_of(scales, code):
 
 
 def check_decode(gpu, code, lens, q_heads, heads, bt, dim, io="f32", seed=0, q_scale=1.0, max_ctx=None,
-                 levels=(-9, -4), scale=0.0, softcap=0.0, window=0, slopes=None, drop=(), q=None):
+                 levels=(-9, -4), scale=0.0, softcap=0.0, window=0, slopes=None, drop=(), q=None, workspace=None):
     rng = np.random.default_rng(seed)
     codes, scales, tables = laid_out(rng, code, lens, heads, bt, dim, levels)
     presents = []
@@ -304,10 +304,10 @@ def check_decode(gpu, code, lens, q_heads, heads, bt, dim, io="f32", seed=0, q_s
     out = torch.full_like(dq, float("nan"))
     options = gpu.ScoreOptions(scale, softcap, window, None if slopes is None else dev(slopes, torch.float32))
     ws = gpu.kv8_decode(cache, dq, dev(tables), dev(np.asarray(lens, np.int32)), out, max_ctx=max_ctx,
-                        options=options)
+                        options=options, workspace=workspace)
     got = out.double().cpu().numpy()
-    if ws is not None:  # the counters, at the end, are back at zero
-        assert not ws[-64:].any()
+    if ws is not None:  # the counters, at the front, are back at zero
+        assert not ws[:16384].any()
     slopes64 = None if slopes is None else np.asarray(slopes, np.float32).astype(np.float64)
     for b, n in enumerate(lens):
         if n <= 0:

@@ -5,7 +5,7 @@ import torch
 
 import kv8_reference as ref
 from kv8_reference import E4M3, INT8
-from test_kv8_gpu import BF16_HALF_STEP, bf16, dev, gpu_cache, laid_out, refused, unit_of, values_of
+from test_kv8_gpu import BF16_HALF_STEP, bf16, check_decode, dev, gpu_cache, laid_out, refused, unit_of, values_of
 
 pytestmark = pytest.mark.gpu
 
@@ -18,7 +18,8 @@ WEIGHT_AND_V = 3 * 2.0 ** -11
 
 
 def check_prefill(gpu, code, shape, seqs, bt, seed=0, q_scale=1.0, scale=0.0, softcap=0.0, window=0, slopes=None,
-                  prefix=None, drop=(), levels=(-9, -4), pad=0, max_rows=None, max_ctx=None, q=None, strided=False):
+                  prefix=None, drop=(), levels=(-9, -4), pad=0, max_rows=None, max_ctx=None, q=None, strided=False,
+                  workspace=None):
     """seqs: (rows, context) of each sequence."""
     q_heads, heads, dim = shape
     rng = np.random.default_rng(seed)
@@ -43,10 +44,10 @@ def check_prefill(gpu, code, shape, seqs, bt, seed=0, q_scale=1.0, scale=0.0, so
     options = gpu.ScoreOptions(scale, softcap, window, None if slopes is None else dev(slopes, torch.float32),
                                None if prefix is None else dev(np.asarray(prefix, np.int32)))
     ws = gpu.kv8_prefill_bf16(cache, dq, dev(tables), dev(np.asarray(lens, np.int32)), dev(starts), out,
-                              max_rows=max_rows, max_ctx=max_ctx, options=options)
+                              max_rows=max_rows, max_ctx=max_ctx, options=options, workspace=workspace)
     got = out.double().cpu().numpy()
     if ws is not None:
-        assert not ws[-64:].any()
+        assert not ws[:16384].any()
     assert (got[starts[-1]:] == -7.0).all()
     slopes64 = None if slopes is None else np.asarray(slopes, np.float32).astype(np.float64)
     for b, (r, c) in enumerate(seqs):
@@ -176,6 +177,19 @@ def test_prefill_of_one_row_is_decode(gpu):
     gpu.kv8_prefill_bf16(cache, q, tables, dlens, dev(np.arange(5, dtype=np.int32)), b)
     # each is within its own bound; bf16's steps are the largest part
     assert ((a.float() - b.float()).abs() <= a.float().abs() * 2.0 ** -7 + a.float().abs().amax() * 2.0 ** -8).all()
+
+
+def test_calls_of_many_shapes_take_turns_in_one_workspace(gpu):
+    ws = torch.full((1 << 26,), 0xff, dtype=torch.uint8, device="cuda")  # only the counters' part starts at zero
+    ws[:16384] = 0
+    for i in range(2):
+        check_decode(gpu, E4M3, [4000 - 900 * i], 16, 2, 16, 64, workspace=ws)
+        check_decode(gpu, INT8, [700, 1, 0, 300 + i] * 24, 8, 8, 32, 128, workspace=ws)
+        check_prefill(gpu, E4M3, (8, 2, 64), [(64, 3000)], 32, workspace=ws)
+        check_decode(gpu, E4M3, list(range(1, 2000, 40)), 4, 4, 16, 64, workspace=ws)
+        check_prefill(gpu, INT8, (4, 1, 128), [(33, 1500), (0, 40), (5, 900 + i)], 16, workspace=ws)
+        check_decode(gpu, E4M3, [2500, 900], 32, 1, 64, 128, io="bf16", workspace=ws)
+    assert not ws[:16384].any()
 
 
 def test_prefill_in_graphs(gpu):
