@@ -103,14 +103,19 @@ struct PairSpan {
     int prefix;
     int tile0, tiles;
 };
-__device__ __forceinline__ PairSpan pair_span(const Kv8PrefillArgs& a, int b, int tile, int tm) {
+// A sequence's rows and lengths: first row, rows, context, prefix.
+__device__ __forceinline__ int4 sequence(const Kv8PrefillArgs& a, int b) {
+    const int r0 = min(max(a.row_starts[b], 0), a.n_rows);
+    const int r1 = min(max(a.row_starts[b + 1], r0), a.n_rows);
+    return int4{r0, r1 - r0, a.ctx_lens[b], a.s.prefix_lens ? a.s.prefix_lens[b] : 0};
+}
+__device__ __forceinline__ PairSpan pair_span(const Kv8PrefillArgs& a, int4 seq, int tile, int tm) {
     PairSpan r;
-    r.row0 = min(max(a.row_starts[b], 0), a.n_rows);
-    r.rows = min(max(a.row_starts[b + 1], r.row0), a.n_rows) - r.row0;
-    const int ctx = a.ctx_lens[b];
-    r.live = max(min(ctx, a.span), 0);
-    r.pos0 = ctx - r.rows;
-    r.prefix = a.s.prefix_lens ? a.s.prefix_lens[b] : 0;
+    r.row0 = seq.x;
+    r.rows = seq.y;
+    r.live = max(min(seq.z, a.span), 0);
+    r.pos0 = seq.z - r.rows;
+    r.prefix = seq.w;
     const int last_pair = min(tile * tm + tm, r.rows * a.group) - 1;
     const int first = r.pos0 + tile * tm / a.group, last = r.pos0 + last_pair / a.group;
     const int end = last < 0 ? 0 : min(max(last + 1, r.prefix), r.live);
@@ -128,11 +133,9 @@ __global__ __launch_bounds__(64 * WAVES, 2 * 4 / WAVES) void kv8_prefill_kernel(
     constexpr int NT = 64 * WAVES;
     constexpr bool PHASES = WAVES == 8;
     constexpr int TM = kWavePairs * WAVES;  // (row, head) pairs per workgroup
-    // K chunks of 16 bytes and V units of 4 tokens by 4 dims, D * 4 of each a
-    // tile: with fewer than threads, one half stages K and the other V
-    constexpr bool APART = 4 * D < NT;
-    constexpr int KL = APART ? 1 : 4 * D / NT;
-    constexpr int VL = KL;
+    // per thread, of a tile's D * 4 K chunks of 16 bytes and V units of 4 tokens by 4 dims
+    constexpr int KL = 4 * D / NT, VL = KL;
+    static_assert(KL * NT == 4 * D, "every thread stages the same");
     __shared__ __attribute__((aligned(16))) unsigned char lds[L::BYTES];
     long long* const sub_off = (long long*)(lds + L::OFF);
     float* const sub_ks = (float*)(lds + L::KS);
@@ -150,17 +153,18 @@ __global__ __launch_bounds__(64 * WAVES, 2 * 4 / WAVES) void kv8_prefill_kernel(
     // ---- this workgroup's sequence, kv head, tile of pairs and piece
     int b = 0, tile = 0, kvh = 0, piece = 0;
     int item;
-    const auto span_of = [&](int b, int tile) { return pair_span(a, b, tile, TM); };
+    PairSpan sp;
     {
         int* const ends = (int*)lds;  // tiles up to and with each sequence
+        int4* const seqs = (int4*)(ends + kSeqsMax);
         int before = 0;
         for (int b0 = 0; b0 < a.batch; b0 += NT) {
             const int s = b0 + tid;
             int x = 0;
             if (s < a.batch) {
-                const int r0 = min(max(a.row_starts[s], 0), a.n_rows);
-                const int r1 = min(max(a.row_starts[s + 1], r0), a.n_rows);
-                x = (int)(((long long)(r1 - r0) * a.group + TM - 1) / TM);
+                const int4 seq = sequence(a, s);
+                seqs[s] = seq;
+                x = (int)(((long long)seq.y * a.group + TM - 1) / TM);
             }
 #pragma unroll
             for (int d = 1; d < 64; d <<= 1) {
@@ -206,25 +210,29 @@ __global__ __launch_bounds__(64 * WAVES, 2 * 4 / WAVES) void kv8_prefill_kernel(
         if (a.batch > 1 && tiles <= kSorted) {
             // several sequences: the longest of all first (a batch of nine, 1-900 rows
             // behind up to 2000 tokens: 200 -> 183 us)
-            int* const length = (int*)lds + kSeqsMax;  // [tiles], zeros to a multiple of 4
-            const int n4 = (tiles + 3) & ~3;
-            for (int i = tid; i < n4; i += NT) {
+            int* const length = (int*)(seqs + kSeqsMax);  // [tiles], zeros to a multiple of 16
+            const int n16 = (tiles + 15) & ~15;
+            for (int i = tid; i < n16; i += NT) {
                 int n = 0;
                 if (i < tiles) {
                     const int s = sequence_of(i);
-                    n = span_of(s, i - (s > 0 ? ends[s - 1] : 0)).tiles + 1;
+                    n = pair_span(a, seqs[s], i - (s > 0 ? ends[s - 1] : 0), TM).tiles + 1;
                 }
                 length[i] = n;
             }
             __syncthreads();
-            for (int i = tid; i < tiles; i += NT) {
+            // four lanes count a tile's rank
+            for (int i = tid >> 2; i < n16; i += NT / 4) {
                 const int mine = length[i];
                 int rank = 0;
-                for (int k = 0; k < n4; k += 4) {
+#pragma unroll 4
+                for (int k = 4 * (tid & 3); k < n16; k += 16) {
                     const int4 n = *(const int4*)(length + k);
                     rank += (n.x > mine || (n.x == mine && k < i)) + (n.y > mine || (n.y == mine && k + 1 < i)) +
                             (n.z > mine || (n.z == mine && k + 2 < i)) + (n.w > mine || (n.w == mine && k + 3 < i));
                 }
+                rank += __shfl_xor(rank, 1);
+                rank += __shfl_xor(rank, 2);
                 if (rank == place) misc[9] = i;
             }
             __syncthreads();
@@ -232,9 +240,13 @@ __global__ __launch_bounds__(64 * WAVES, 2 * 4 / WAVES) void kv8_prefill_kernel(
         }
         b = __builtin_amdgcn_readfirstlane(sequence_of(t));
         tile = __builtin_amdgcn_readfirstlane(t - (b > 0 ? ends[b - 1] : 0));
+        const int4 seq = seqs[b];
+        sp = pair_span(a,
+                       int4{__builtin_amdgcn_readfirstlane(seq.x), __builtin_amdgcn_readfirstlane(seq.y),
+                            __builtin_amdgcn_readfirstlane(seq.z), __builtin_amdgcn_readfirstlane(seq.w)},
+                       tile, TM);
         __syncthreads();
     }
-    const PairSpan sp = span_of(b, tile);
     const int row0 = sp.row0, rows = sp.rows, live = sp.live, pos0 = sp.pos0, prefix = sp.prefix;
     const int pairs = rows * a.group;
     const int32_t* table = a.tables + (long long)b * a.max_blocks;
@@ -282,11 +294,14 @@ __global__ __launch_bounds__(64 * WAVES, 2 * 4 / WAVES) void kv8_prefill_kernel(
     }
     // bounds of the wavefront's pairs together, for whole tiles
     int w_lo = 0, w_hi = 0;
+    int q_lo, q_hi;  // first and last position of the wavefront's rows
     {
         const int x0 = min(tile * TM + wave * kWavePairs, pairs - 1) / a.group;
         const int x1 = min(tile * TM + wave * kWavePairs + kWavePairs - 1, pairs - 1) / a.group;
-        w_hi = pos0 + x0 < 0 ? 0 : min(max(pos0 + x0 + 1, prefix), live);   // smallest end
-        w_lo = a.s.window > 0 ? max(pos0 + x1 - a.s.window + 1, 0) : 0;      // largest begin
+        q_lo = pos0 + x0;
+        q_hi = pos0 + x1;
+        w_hi = q_lo < 0 ? 0 : min(max(q_lo + 1, prefix), live);      // smallest end
+        w_lo = a.s.window > 0 ? max(q_hi - a.s.window + 1, 0) : 0;   // largest begin
     }
 
     float16_t o[DT];
@@ -336,10 +351,8 @@ __global__ __launch_bounds__(64 * WAVES, 2 * 4 / WAVES) void kv8_prefill_kernel(
     constexpr int CPR = D / 16;
     // V unit u: four tokens from 4 tg on, four dims from 4 (vc + 8 u) on.  Of a
     // wavefront's stores to V^T, 8 bytes a lane, 32 lanes then cover every bank twice.
-    const bool stages_k = !APART || !second, stages_v = !APART || second;
-    const int vwave = APART ? wave & (WAVES / 2 - 1) : wave;
-    const int tg = ((lane >> 2) & 7) + 8 * (vwave & 1);
-    const int vc = (lane & 3) + 4 * (lane >> 5) + 8 * VL * (vwave >> 1);
+    const int tg = ((lane >> 2) & 7) + 8 * (wave & 1);
+    const int vc = (lane & 3) + 4 * (lane >> 5) + 8 * VL * (wave >> 1);
     // what the next loads and weights need of the table, read ahead of them
     long long koff[KL], voff = 0;
     float vnext = 0.f;
@@ -353,7 +366,6 @@ __global__ __launch_bounds__(64 * WAVES, 2 * 4 / WAVES) void kv8_prefill_kernel(
         vnext = sub_vs[4 * x + (tg >> 2)];
     };
     auto load_k = [&]() __attribute__((always_inline)) {
-        if (!stages_k) return;
 #pragma unroll
         for (int u = 0; u < KL; u++) {
             const int tk = (tid + NT * u) / CPR;
@@ -361,7 +373,6 @@ __global__ __launch_bounds__(64 * WAVES, 2 * 4 / WAVES) void kv8_prefill_kernel(
         }
     };
     auto load_v = [&]() __attribute__((always_inline)) {
-        if (!stages_v) return;
         vsc = vnext;
         const uint8_t* vb = a.c.v + voff + (tg & 3) * 4 * D + 4 * vc;
 #pragma unroll
@@ -370,7 +381,6 @@ __global__ __launch_bounds__(64 * WAVES, 2 * 4 / WAVES) void kv8_prefill_kernel(
             for (int i = 0; i < 4; i++) vst[u][i] = *(const uint32_t*)(vb + i * D + 32 * u);
     };
     auto store_k = [&](int it) __attribute__((always_inline)) {
-        if (!stages_k) return;
         unsigned char* ks = kslot0 + (it & 1) * L::KBYTES;
 #pragma unroll
         for (int u = 0; u < KL; u++) {
@@ -393,7 +403,6 @@ __global__ __launch_bounds__(64 * WAVES, 2 * 4 / WAVES) void kv8_prefill_kernel(
         return any_gone ? __builtin_amdgcn_readfirstlane((int)((sub_gone[x >> 3] >> (4 * (x & 7))) & 15)) : 0;
     };
     auto store_v = [&](int t0, int it, int x, float unit) __attribute__((always_inline)) {
-        if (!stages_v) return;
         const int key = (t0 + x) * kKeys;
         const int gone = gone_of(x);
         if (gone || key + kKeys > live) {
@@ -469,30 +478,35 @@ __global__ __launch_bounds__(64 * WAVES, 2 * 4 / WAVES) void kv8_prefill_kernel(
     };
     auto ready = [&](float16_t& st, Factors& w, int t0, int x, int kb, bool edge) __attribute__((always_inline)) {
         const int k0 = (t0 + x) * kKeys + 32 * kb + 4 * h;
-        w.sb = w.sl = 0.f;
+        w.sb = CAP ? a.s.cap_log2 : 0.f;
+        w.sl = 0.f;
 #pragma unroll
         for (int u = 0; u < 2; u++) w.f[u] = ks4[2 * kb + u] * crow;
         if constexpr (CAP) {
-            // cap tanh(x) = cap - 2 cap / (e^2x + 1)
+            // cap tanh(x) = cap - 2 cap / (e^2x + 1), linear in what is kept of it
 #pragma unroll
             for (int r = 0; r < 16; r++)
-                st[r] = __builtin_fmaf(-2.f * a.s.cap_log2,
-                                       __builtin_amdgcn_rcpf(
-                                           __builtin_amdgcn_exp2f(st[r] * (w.f[r >> 3] * 2.885390081777927f)) + 1.f),
-                                       a.s.cap_log2);
-            w.f[0] = w.f[1] = 1.f;
+                st[r] = __builtin_amdgcn_rcpf(
+                    __builtin_amdgcn_exp2f(st[r] * (w.f[r >> 3] * 2.885390081777927f)) + 1.f);
+            w.f[0] = w.f[1] = -2.f * a.s.cap_log2;
         }
         if constexpr (BIAS) {
-            w.sl = slope;
-            w.sb = slope * (float)(k0 - qpos);
-            if (a.s.prefix_lens) {  // keys on both sides of the row
+            // keys in front of all rows, behind all of them (a prefix's), or some on
+            // either side (a batch of nine, 1-900 rows behind prefixes: 149 us with
+            // every tile by the third way, 132 with the three)
+            const int kt = (t0 + x) * kKeys;
+            const bool behind = kt >= q_hi;
+            w.sl = behind ? -slope : slope;
+            if (prefix > q_lo && kt + kKeys - 1 > q_lo && !behind) {
                 asm volatile("");
 #pragma unroll
                 for (int r = 0; r < 16; r++)
                     st[r] = __builtin_fmaf(-slope, fabsf((float)(k0 - qpos) + (float)(8 * (r >> 2) + (r & 3))),
                                            st[r] * w.f[r >> 3]);
                 w.f[0] = w.f[1] = 1.f;
-                w.sl = w.sb = 0.f;
+                w.sl = 0.f;
+            } else {
+                w.sb = __builtin_fmaf(w.sl, (float)(k0 - qpos), w.sb);
             }
         }
         if (edge) {
@@ -541,7 +555,7 @@ __global__ __launch_bounds__(64 * WAVES, 2 * 4 / WAVES) void kv8_prefill_kernel(
 #pragma unroll
                 for (int r = 0; r < 16; r++) {
                     const float bias =
-                        BIAS ? __builtin_fmaf(w[kb].sl, (float)(8 * (r >> 2) + (r & 3)), w[kb].sb) : 0.f;
+                        BIAS ? __builtin_fmaf(w[kb].sl, (float)(8 * (r >> 2) + (r & 3)), w[kb].sb) : w[kb].sb;
                     top = fmaxf(top, __builtin_fmaf(st[kb][r], w[kb].f[r >> 3], bias));
                 }
             // only this pair's own sum moves it: a pair's result is its own, whatever
@@ -940,12 +954,14 @@ int nyion_kv8_prefill_attention_bf16(const nyion_kv8_cache* cache, const int32_t
         auto launch = [&](auto d, auto code, auto cap, auto bias) {
             constexpr int D = decltype(d)::value, CODE = decltype(code)::value;
             constexpr bool CAP = decltype(cap)::value, BIAS = decltype(bias)::value;
-            if (p.waves == 8)
-                hipLaunchKernelGGL((kv8_prefill_kernel<D, CODE, CAP, BIAS, 8>), dim3(grid), dim3(512), 0,
-                                   (hipStream_t)stream, a);
-            else
-                hipLaunchKernelGGL((kv8_prefill_kernel<D, CODE, CAP, BIAS, 4>), dim3(grid), dim3(256), 0,
-                                   (hipStream_t)stream, a);
+            if constexpr (D == 128)
+                if (p.waves == 8) {
+                    hipLaunchKernelGGL((kv8_prefill_kernel<D, CODE, CAP, BIAS, 8>), dim3(grid), dim3(512), 0,
+                                       (hipStream_t)stream, a);
+                    return;
+                }
+            hipLaunchKernelGGL((kv8_prefill_kernel<D, CODE, CAP, BIAS, 4>), dim3(grid), dim3(256), 0,
+                               (hipStream_t)stream, a);
         };
         auto by_options = [&](auto d, auto code) {
             if (a.s.cap_log2 > 0.f && a.s.slopes)
