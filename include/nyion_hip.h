@@ -713,7 +713,8 @@ int nyion_kv8_decode_attention(const nyion_kv8_cache* cache, const int32_t* bloc
  * from 0) of q [n_rows][n_heads][head_dim] are the last tokens of sequence b,
  * row r at position ctx_lens[b] - row_starts[b + 1] + r; their K/V are in the
  * cache already.  Rows behind row_starts[batch] are left as they are in out,
- * and rows at negative positions give zeros.  max_rows and max_ctx, bounds of
+ * rows of row_starts behind n_rows are not computed, and rows at negative
+ * positions give zeros.  max_rows and max_ctx, bounds of
  * the rows and the length of one sequence, shape the launch and the
  * workspace, not the result.  q is carried exactly (bf16 relative to the
  * row's largest value in binary16), weights and V in binary16 (11 bits), sums

@@ -451,6 +451,9 @@ int kv8_score_args(ScoreArgs& s, const nyion_score_options* o, int head_dim, boo
     const double log2e = 1.4426950408889634;
     s.scale_log2 = (float)(o->softcap > 0.f ? scale / o->softcap : scale * log2e);
     s.cap_log2 = (float)(o->softcap * log2e);
+    if (!isfinite(s.scale_log2) || !isfinite(s.cap_log2))
+        return set_error(NYION_ERR_INVALID, "%s: scale %g with softcap %g leaves f32's range", what, scale,
+                         (double)o->softcap);
     s.window = o->window > 0 ? std::min(o->window, 1 << 30) : 0;  // sums with a position stay in 32 bits
     s.slopes = o->slopes;
     s.prefix_lens = o->prefix_lens;
@@ -541,7 +544,7 @@ int nyion_kv8_write(const nyion_kv8_cache* cache, const int64_t* slots, int n_ro
     if ((long long)n_rows * per > 16384) a.span = std::min(bt, 64);
     const long long units = (long long)((n_rows + a.span - 1) / a.span) * per;
     const long long grid = (units + teams - 1) / teams;
-    if (grid > INT_MAX) return set_error(NYION_ERR_UNSUPPORTED, "%s: n_rows %d", what, n_rows);
+    if (units > INT_MAX) return set_error(NYION_ERR_UNSUPPORTED, "%s: n_rows %d", what, n_rows);
     auto launch = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(256), 0, (hipStream_t)stream, a);
     };

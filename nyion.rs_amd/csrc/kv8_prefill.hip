@@ -95,30 +95,32 @@ __device__ __forceinline__ float sum_half(float v) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// A sequence's rows and lengths.
+struct Rows {
+    int row0, rows;  // of those that q holds
+    int pos0;        // position of row0
+    int live, prefix;
+};
+__device__ __forceinline__ Rows rows_of(const Kv8PrefillArgs& a, int b) {
+    Rows s;
+    const int end = a.row_starts[b + 1], ctx = a.ctx_lens[b];
+    s.row0 = min(max(a.row_starts[b], 0), a.n_rows);
+    s.rows = min(max(end, s.row0), a.n_rows) - s.row0;
+    s.pos0 = (int)((unsigned)ctx - (unsigned)end + (unsigned)s.row0);
+    s.live = max(min(ctx, a.span), 0);
+    s.prefix = a.s.prefix_lens ? a.s.prefix_lens[b] : 0;
+    return s;
+}
+
 // The keys that a tile of pairs sees, as tiles of kKeys.
 struct PairSpan {
-    int row0, rows;  // of the sequence
-    int live;        // its keys that can be read
-    int pos0;        // position of its row 0
-    int prefix;
     int tile0, tiles;
 };
-// A sequence's rows and lengths: first row, rows, context, prefix.
-__device__ __forceinline__ int4 sequence(const Kv8PrefillArgs& a, int b) {
-    const int r0 = min(max(a.row_starts[b], 0), a.n_rows);
-    const int r1 = min(max(a.row_starts[b + 1], r0), a.n_rows);
-    return int4{r0, r1 - r0, a.ctx_lens[b], a.s.prefix_lens ? a.s.prefix_lens[b] : 0};
-}
-__device__ __forceinline__ PairSpan pair_span(const Kv8PrefillArgs& a, int4 seq, int tile, int tm) {
+__device__ __forceinline__ PairSpan pair_span(const Kv8PrefillArgs& a, const Rows& s, int tile, int tm) {
     PairSpan r;
-    r.row0 = seq.x;
-    r.rows = seq.y;
-    r.live = max(min(seq.z, a.span), 0);
-    r.pos0 = seq.z - r.rows;
-    r.prefix = seq.w;
-    const int last_pair = min(tile * tm + tm, r.rows * a.group) - 1;
-    const int first = r.pos0 + tile * tm / a.group, last = r.pos0 + last_pair / a.group;
-    const int end = last < 0 ? 0 : min(max(last + 1, r.prefix), r.live);
+    const int last_pair = min(tile * tm + tm, s.rows * a.group) - 1;
+    const int first = s.pos0 + tile * tm / a.group, last = s.pos0 + last_pair / a.group;
+    const int end = last < 0 ? 0 : min(max(last + 1, s.prefix), s.live);
     const int begin = a.s.window > 0 ? min(max(first - a.s.window + 1, 0), end) : 0;
     r.tile0 = begin / kKeys;
     r.tiles = (end + kKeys - 1) / kKeys - r.tile0;
@@ -126,7 +128,8 @@ __device__ __forceinline__ PairSpan pair_span(const Kv8PrefillArgs& a, int4 seq,
 }
 
 template <int D, int CODE, bool CAP, bool BIAS, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, 2 * 4 / WAVES) void kv8_prefill_kernel(Kv8PrefillArgs a) {
+__global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 1 : D == 128 ? 2 : 3) void
+kv8_prefill_kernel(Kv8PrefillArgs a) {
     using L = Kv8Lds<D>;
     constexpr int DT = D / 32;       // 32-dim tiles of O^T
     constexpr int KS = D / 16;       // k-steps of the S product
@@ -135,6 +138,7 @@ __global__ __launch_bounds__(64 * WAVES, 2 * 4 / WAVES) void kv8_prefill_kernel(
     constexpr int TM = kWavePairs * WAVES;  // (row, head) pairs per workgroup
     // per thread, of a tile's D * 4 K chunks of 16 bytes and V units of 4 tokens by 4 dims
     constexpr int KL = 4 * D / NT, VL = KL;
+    static_assert((kSeqsMax * (1 + sizeof(Rows) / 4) + kSorted) * 4 <= L::TILES, "the selection's lists");
     static_assert(KL * NT == 4 * D, "every thread stages the same");
     __shared__ __attribute__((aligned(16))) unsigned char lds[L::BYTES];
     long long* const sub_off = (long long*)(lds + L::OFF);
@@ -154,17 +158,18 @@ __global__ __launch_bounds__(64 * WAVES, 2 * 4 / WAVES) void kv8_prefill_kernel(
     int b = 0, tile = 0, kvh = 0, piece = 0;
     int item;
     PairSpan sp;
+    Rows seq;
     {
         int* const ends = (int*)lds;  // tiles up to and with each sequence
-        int4* const seqs = (int4*)(ends + kSeqsMax);
+        Rows* const seqs = (Rows*)(ends + kSeqsMax);
         int before = 0;
         for (int b0 = 0; b0 < a.batch; b0 += NT) {
             const int s = b0 + tid;
             int x = 0;
             if (s < a.batch) {
-                const int4 seq = sequence(a, s);
-                seqs[s] = seq;
-                x = (int)(((long long)seq.y * a.group + TM - 1) / TM);
+                const Rows mine = rows_of(a, s);
+                seqs[s] = mine;
+                x = (int)(((long long)mine.rows * a.group + TM - 1) / TM);
             }
 #pragma unroll
             for (int d = 1; d < 64; d <<= 1) {
@@ -240,14 +245,15 @@ __global__ __launch_bounds__(64 * WAVES, 2 * 4 / WAVES) void kv8_prefill_kernel(
         }
         b = __builtin_amdgcn_readfirstlane(sequence_of(t));
         tile = __builtin_amdgcn_readfirstlane(t - (b > 0 ? ends[b - 1] : 0));
-        const int4 seq = seqs[b];
-        sp = pair_span(a,
-                       int4{__builtin_amdgcn_readfirstlane(seq.x), __builtin_amdgcn_readfirstlane(seq.y),
-                            __builtin_amdgcn_readfirstlane(seq.z), __builtin_amdgcn_readfirstlane(seq.w)},
-                       tile, TM);
+        seq.row0 = __builtin_amdgcn_readfirstlane(seqs[b].row0);
+        seq.rows = __builtin_amdgcn_readfirstlane(seqs[b].rows);
+        seq.pos0 = __builtin_amdgcn_readfirstlane(seqs[b].pos0);
+        seq.live = __builtin_amdgcn_readfirstlane(seqs[b].live);
+        seq.prefix = __builtin_amdgcn_readfirstlane(seqs[b].prefix);
+        sp = pair_span(a, seq, tile, TM);
         __syncthreads();
     }
-    const int row0 = sp.row0, rows = sp.rows, live = sp.live, pos0 = sp.pos0, prefix = sp.prefix;
+    const int row0 = seq.row0, rows = seq.rows, live = seq.live, pos0 = seq.pos0, prefix = seq.prefix;
     const int pairs = rows * a.group;
     const int32_t* table = a.tables + (long long)b * a.max_blocks;
     const int n_pieces = max(min(a.pieces, sp.tiles / kPieceTiles), 1);

@@ -237,6 +237,16 @@ def test_write_of_runs_that_windows_cut(gpu, bt):
     run_write(gpu, E4M3, 300 if bt == 16 else 9, 4, bt, 64, slots, x, "bf16")
 
 
+@pytest.mark.parametrize("bt", [16, 128])
+@pytest.mark.parametrize("code", [E4M3, INT8])
+def test_write_of_a_slot_twice(gpu, code, bt):
+    """Each is a run of its own; a later one finds the tokens in front of it as the earlier left them."""
+    rng = np.random.default_rng(88)
+    slots = np.array([5, 6, 6, 7, 7, 7, bt + 3, bt, bt, bt + 1], np.int64)
+    x = [rng.standard_normal((len(slots), 2, 64)) * np.exp2(rng.integers(-6, 7, (len(slots), 1, 1))) for _ in range(2)]
+    run_write(gpu, code, 4, 2, bt, 64, slots, x, "f32")
+
+
 def test_write_skips_slots_outside_the_cache(gpu):
     rng = np.random.default_rng(10)
     slots = [-1, 5, 6, 64, 2 ** 40, -2 ** 40, 63, 7, 8]
@@ -583,6 +593,8 @@ def test_refusals(gpu):
     refused(gpu, INV, lambda: dec(max_ctx=0))
     refused(gpu, INV, lambda: dec(options=gpu.ScoreOptions(softcap=-1.0)))
     refused(gpu, INV, lambda: dec(options=gpu.ScoreOptions(scale=float("nan"))))
+    refused(gpu, INV, lambda: dec(options=gpu.ScoreOptions(softcap=1e-42)))
+    refused(gpu, INV, lambda: dec(options=gpu.ScoreOptions(scale=3e38)))
     refused(gpu, INV, lambda: dec(options=gpu.ScoreOptions(prefix_lens=lens)))
     refused(gpu, INV, lambda: dec(options=gpu.ScoreOptions(slopes=torch.zeros(7, device="cuda"))))
     wide = torch.zeros(2, 8 * 64 + 2, device="cuda")

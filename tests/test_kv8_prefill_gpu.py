@@ -122,6 +122,20 @@ def test_prefill_does_not_depend_on_its_bounds(gpu):
         check_prefill(gpu, E4M3, (8, 2, 64), [(90, 1900), (33, 33)], 16, max_rows=max_rows, max_ctx=max_ctx)
 
 
+@pytest.mark.parametrize("held", [1, 31, 32, 70, 71])
+def test_prefill_of_fewer_rows_than_the_starts_tell(gpu, held):
+    """Positions go by row_starts: the rows that q holds are those of the whole batch."""
+    rng = np.random.default_rng(40)
+    lens = [90, 200, 64]
+    codes, scales, tables = laid_out(rng, E4M3, lens, 2, 16, 64)
+    cache, q = gpu_cache(gpu, codes, scales, E4M3), torch.randn(102, 8, 64, device="cuda").bfloat16()
+    starts, dlens = dev(np.array([0, 31, 71, 102], np.int32)), dev(np.asarray(lens, np.int32))
+    whole, part = torch.empty_like(q), torch.full_like(q, -7.0)
+    gpu.kv8_prefill_bf16(cache, q, dev(tables), dlens, starts, whole)
+    gpu.kv8_prefill_bf16(cache, q[:held], dev(tables), dlens, starts, part[:held])
+    assert torch.equal(part[:held], whole[:held]) and (part[held:] == -7.0).all()
+
+
 def test_prefill_skips_pages_that_are_no_blocks(gpu):
     for drop in ([(1, -1)], [(0, 2 ** 31 - 1), (5, -7)], [(4, 10 ** 6), (5, -1), (6, -1), (7, -1)],
                  [(i, -1) for i in range(100)]):
