@@ -499,20 +499,24 @@ kv8_prefill_kernel(Kv8PrefillArgs a) {
         if constexpr (BIAS) {
             // keys in front of all rows, behind all of them (a prefix's), or some on
             // either side (a batch of nine, 1-900 rows behind prefixes: 149 us with
-            // every tile by the third way, 132 with the three)
+            // every tile by the last way, 133 with the three)
+            w.sl = slope;
+            w.sb = __builtin_fmaf(slope, (float)(k0 - qpos), w.sb);
             const int kt = (t0 + x) * kKeys;
-            const bool behind = kt >= q_hi;
-            w.sl = behind ? -slope : slope;
-            if (prefix > q_lo && kt + kKeys - 1 > q_lo && !behind) {
+            if (prefix > q_lo && kt + kKeys - 1 > q_lo) {
                 asm volatile("");
+                if (kt >= q_hi) {
+                    w.sl = -slope;
+                    w.sb = __builtin_fmaf(-slope, (float)(k0 - qpos), CAP ? a.s.cap_log2 : 0.f);
+                } else {
 #pragma unroll
-                for (int r = 0; r < 16; r++)
-                    st[r] = __builtin_fmaf(-slope, fabsf((float)(k0 - qpos) + (float)(8 * (r >> 2) + (r & 3))),
-                                           st[r] * w.f[r >> 3]);
-                w.f[0] = w.f[1] = 1.f;
-                w.sl = 0.f;
-            } else {
-                w.sb = __builtin_fmaf(w.sl, (float)(k0 - qpos), w.sb);
+                    for (int r = 0; r < 16; r++)
+                        st[r] = __builtin_fmaf(-slope, fabsf((float)(k0 - qpos) + (float)(8 * (r >> 2) + (r & 3))),
+                                               st[r] * w.f[r >> 3]);
+                    w.f[0] = w.f[1] = 1.f;
+                    w.sl = 0.f;
+                    w.sb = CAP ? a.s.cap_log2 : 0.f;
+                }
             }
         }
         if (edge) {
