@@ -41,9 +41,10 @@ constexpr int kKeys = 64;          // per tile
 constexpr int kWavePairs = 32;     // pairs per wavefront
 constexpr int kTableTiles = 128;   // tiles of the page table in LDS
 constexpr int kSeqsMax = 1024;     // sequences per launch
-constexpr int kSorted = 512;       // tiles of a kv head that are put in order of their lengths
-constexpr int kPieceTiles = 4;   // fewest tiles of a piece
-constexpr int kMaxPieces = 16;   // the join walks them one by one
+constexpr int kSorted = 512;       // tiles of a kv head that are put in order of their lengths,
+constexpr int kSortedItems = 6144;  // of launches of about three rounds: 768 workgroups of eight wavefronts
+constexpr int kPieceTiles = 4;     // fewest tiles of a piece
+constexpr int kMaxPieces = 16;     // the join walks them one by one
 constexpr float kSumLimit = 16384.f;
 constexpr float kVUnit = 64.f;     // 448 * 64 stays below binary16's largest
 constexpr float kVLeast = 7.888609052210118e-31f;  // 2^-100
@@ -212,9 +213,11 @@ kv8_prefill_kernel(Kv8PrefillArgs a) {
             return lo;
         };
         int t = tiles - 1 - place;  // later tiles of a sequence are longer: first
-        if (a.batch > 1 && tiles <= kSorted) {
+        if (a.batch > 1 && tiles <= kSorted && tiles * a.c.n_kv_heads <= kSortedItems / WAVES) {
             // several sequences: the longest of all first (a batch of nine, 1-900 rows
-            // behind up to 2000 tokens: 200 -> 183 us)
+            // behind up to 2000 tokens: 134 -> 127 us, one of 40, 4-200 rows: 136 -> 126;
+            // what it costs shows where all lengths are the same, 16 of 300 rows: 95 -> 103,
+            // and where many rounds even the lengths out, 128 of 1-100: 192 -> 201)
             int* const length = (int*)(seqs + kSeqsMax);  // [tiles], zeros to a multiple of 16
             const int n16 = (tiles + 15) & ~15;
             for (int i = tid; i < n16; i += NT) {
@@ -863,12 +866,21 @@ static int prefill_plan(Kv8PrefillPlan& p, const Kv8& c, int batch, int n_heads,
     };
     const long long cus = device_cu_count();
     // Eight wavefronts in two phases at head_dim 128 where they give every CU two
-    // workgroups or more in turn, four without phases elsewhere.  Measured (us, four /
-    // eight; 32/8 heads of 128): 8192 rows (1024 workgroups of eight) 615 / 552, 4096
-    // (512) 176 / 149, four sequences of 1500 behind 500 (768) 185 / 167, 3000 (375) 108 /
-    // 127, 2048 (256) 61 / 76; 32/4 heads of 64, whose products are too short to hide the
-    // other phase, 8192 rows 443 / 537.
-    p.waves = c.head_dim == 128 && items(8) >= 2 * cus ? 8 : 4;
+    // workgroups or more in turn, in rounds that are nearly full and tiles that are not
+    // much emptier than those of four; four without phases elsewhere.  Counted as for
+    // sequences of equal rows.  Measured (us, four / eight; 32/8 heads of 128): 8192 rows
+    // (1024 workgroups of eight) 608 / 555, 4096 (512) 171 / 154, four sequences of 1500
+    // behind 500 (768) 187 / 172; 3000 rows (375) 108 / 127; nine of 1-900 (576: two rounds
+    // and a quarter) 127 / 134; 64 of 16 behind 2000 (512, a quarter full) 94 / 154, of 40
+    // behind 1000 (512) 109 / 100; 32/4 heads of 64, whose products are too short to hide
+    // the other phase, 8192 rows 443 / 537.
+    const auto tiles_of = [&](int waves) {
+        const long long each = ((long long)n_rows * group + batch - 1) / batch, tm = kWavePairs * waves;
+        return (each + tm - 1) / tm * p.chunk * c.n_kv_heads;
+    };
+    const long long n8 = tiles_of(8), rounds = (n8 + cus - 1) / cus;
+    const bool full = 8 * n8 >= 7 * rounds * cus && 20 * n8 <= 11 * tiles_of(4);
+    p.waves = c.head_dim == 128 && n8 >= 2 * cus && full ? 8 : 4;
     const int tm = kWavePairs * p.waves;
     p.items = items(p.waves);
     if (p.items >= (1 << 24)) return set_error(NYION_ERR_UNSUPPORTED, "%s: %lld tiles", what, p.items);

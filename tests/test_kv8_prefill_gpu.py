@@ -100,6 +100,31 @@ def test_prefill_options(gpu, code, options):
     check_prefill(gpu, code, (8, 4, 128), [(70, 200), (64, 64), (30, 300), (1, 5)], 32, **o)
 
 
+@pytest.mark.parametrize("code,softcap", [(E4M3, 0.0), (INT8, 20.0)])
+@pytest.mark.parametrize("shape", [(2, 1, 64), (2, 2, 128)])
+def test_prefill_of_biased_rows_within_prefixes(gpu, code, softcap, shape):
+    """Keys in front of a wavefront's rows, around them and behind all of them."""
+    slopes = 2.0 ** (-8.0 * np.arange(1, 3) / 2)
+    check_prefill(gpu, code, shape, [(300, 420), (90, 400), (64, 640)], 16, slopes=slopes, softcap=softcap,
+                  prefix=[400, 390, 640])
+
+
+@pytest.mark.parametrize("code", [E4M3, INT8])
+@pytest.mark.parametrize("options", [
+    dict(), dict(softcap=30.0), dict(slopes=True), dict(slopes=True, softcap=20.0, window=100),
+    dict(slopes=True, prefix=True), dict(drop=[(1, -1)])])
+def test_prefill_of_many_tiles(gpu, code, options):
+    """Launches that workgroups of eight wavefronts take, in whole tiles and with ragged ends."""
+    rng = np.random.default_rng(12)
+    rows = [32] * 30 + [33, 1, 31, 60, 35] + [32] * 29
+    o = dict(options)
+    if o.get("slopes"):
+        o["slopes"] = 2.0 ** (-8.0 * np.arange(1, 65) / 64)
+    if o.get("prefix"):
+        o["prefix"] = rng.integers(0, 150, len(rows)).tolist()
+    check_prefill(gpu, code, (64, 8, 128), [(r, r + int(n)) for r, n in zip(rows, rng.integers(0, 150, len(rows)))], 16, **o)
+
+
 @pytest.mark.parametrize("shape", [(32, 4, 64), (8, 2, 128)])
 @pytest.mark.parametrize("seqs", [[(3, 5000)], [(40, 9000)], [(1, 3000), (16, 2000), (1, 1)], [(300, 8500)]])
 def test_prefill_with_the_keys_cut_into_pieces(gpu, shape, seqs):
@@ -160,6 +185,28 @@ def test_prefill_of_long_ranges(gpu):
     """More keys than one table of pages holds."""
     check_prefill(gpu, E4M3, (1, 1, 64), [(2, 17000)], 16, max_ctx=64)
     check_prefill(gpu, E4M3, (1, 1, 128), [(70, 8400)], 64, max_ctx=64)
+
+
+def test_prefill_of_long_ranges_in_many_tiles(gpu):
+    """The same by workgroups of eight wavefronts: sequences that share their pages, of many heads, three of which
+    are compared."""
+    rng = np.random.default_rng(50)
+    heads, ctx, rows = 64, 8400, [129, 150, 130, 256, 140, 200, 129, 180]
+    codes, scales, tables = laid_out(rng, E4M3, [ctx], heads, 64, 128)
+    starts = np.concatenate(([0], np.cumsum(rows))).astype(np.int32)
+    q = torch.randn(int(starts[-1]), heads, 128, device="cuda").bfloat16()
+    out = torch.empty_like(q)
+    lens = np.array([ctx - 30 * b for b in range(len(rows))], np.int32)
+    gpu.kv8_prefill_bf16(gpu_cache(gpu, codes, scales, E4M3), q, dev(np.repeat(tables, len(rows), 0)), dev(lens),
+                         dev(starts), out)
+    for b, h in ((0, 0), (3, 17), (7, 63)):
+        at, n = slice(starts[b], starts[b + 1]), int(lens[b])
+        k, v = values_of(codes[:, :, h:h + 1], scales[:, :, h:h + 1], E4M3, tables[0], n, 64)
+        qh, pos = q[at, h:h + 1].double().cpu().numpy(), n - rows[b] + np.arange(rows[b])
+        want, bound = ref.attention(qh, k, v, pos, unit=unit_of(scales[:, :, h:h + 1], E4M3) * 2.0 ** 15)
+        spread, _ = ref.attention(qh, k, np.abs(v), pos)
+        err = np.abs(out[at, h:h + 1].double().cpu().numpy() - want)
+        assert (err <= bound + spread * WEIGHT_AND_V + np.abs(want) * BF16_HALF_STEP + 2.0 ** -133).all()
 
 
 def test_prefill_of_rows_of_a_wider_projection(gpu):
