@@ -36,8 +36,11 @@
 // L2s, which the XCDs do not share) and the last one to arrive joins them in
 // the order of the pieces, so that the order of arrival changes nothing.
 //
-// Bound: the cache's bytes at batch, the chain length -> table -> rows ->
-// partials -> join for single sequences.
+// Bound: the cache's bytes at batch (64 sequences of 16640 tokens, 32/4 heads of
+// 64: 104 us, 5.25 TB/s, where the same kernel without its products takes 103;
+// 24 of 200-16000, 32/8 of 128: 87 us, 4.6 TB/s, with capped scores 96); for single
+// sequences the chain length -> table -> rows -> partials -> join (32 tokens to
+// 128: 4.7 us; 4096 of 4 kv heads of 64: 9.3 us; 32768: 15.5 us).
 #include <limits.h>
 
 #include <algorithm>

@@ -3,8 +3,8 @@
 // Sequence b brings rows_b query rows, the last tokens of its context, and
 // each kv head is read by `group` q heads.  The rows_b * group (row, head)
 // pairs of a kv head are numbered row-major, whatever the group's size, and cut
-// into tiles; a workgroup of four wavefronts takes one tile of 128 pairs, 32 a
-// wavefront, through the keys that its rows see, 64 at a time:
+// into tiles; a workgroup takes one tile, 32 pairs for each of its four or
+// eight wavefronts, through the keys that its rows see, 64 at a time:
 //   S^T[32 keys][32 pairs] += K . Q^T    v_mfma_f32_32x32x16_f16
 //   O^T[32 dims][32 pairs] += V^T . P^T  v_mfma_f32_32x32x16_f16
 // The result layout of S^T (a lane holds one pair and 16 keys) is the B
@@ -19,6 +19,11 @@
 // reach so that binary16 holds them; K's into the scores' factor, which the
 // exponential's FMA takes anyway.
 //
+// Eight wavefronts work in two halves, a phase apart: while one half's products
+// keep the matrix unit busy, the other takes exponentials and stages the next
+// tile, one wavefront of each half on a SIMD.  Four have no phases; two
+// workgroups (three at head_dim 64) on a CU overlap as they happen to.
+//
 // Pages: a table of 128 tiles (512 subtiles of 16 tokens, each in one block)
 // is kept in LDS, the place and the scales of each subtile, so that the loads
 // of a tile wait for nothing but LDS; longer ranges refill it.
@@ -28,6 +33,12 @@
 //
 // Few tiles: their keys are cut into pieces as well, joined through the
 // workspace by the last piece to arrive, in the order of the pieces.
+//
+// Bound: the matrix unit and the power that it may draw for large launches
+// (8192 rows of 32/8 heads of 128: 534-565 us, 0.97-1.03 PFLOP/s, where a large
+// library product reaches 1.21; 450 us with all data zero); with capped scores
+// the exponentials (705 us); for smaller ones what a workgroup does besides its
+// tiles, 7 us to find and fetch the first of them, and rounds that are not full.
 #include <limits.h>
 
 #include <algorithm>
@@ -41,8 +52,10 @@ constexpr int kKeys = 64;          // per tile
 constexpr int kWavePairs = 32;     // pairs per wavefront
 constexpr int kTableTiles = 128;   // tiles of the page table in LDS
 constexpr int kSeqsMax = 1024;     // sequences per launch
-constexpr int kSorted = 512;       // tiles of a kv head that are put in order of their lengths,
-constexpr int kSortedItems = 6144;  // of launches of about three rounds: 768 workgroups of eight wavefronts
+// Tiles of a kv head that are put in order of their lengths at most, and wavefronts
+// of such a launch: about three rounds.
+constexpr int kSorted = 512;
+constexpr int kSortedItems = 6144;
 constexpr int kPieceTiles = 4;     // fewest tiles of a piece
 constexpr int kMaxPieces = 16;     // the join walks them one by one
 constexpr float kSumLimit = 16384.f;
@@ -153,7 +166,7 @@ kv8_prefill_kernel(Kv8PrefillArgs a) {
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int j = lane & 31;
     const int h = lane >> 5;
-    const bool second = wave >= WAVES / 2;  // half of the workgroup, a phase behind the other
+    const bool second = wave >= WAVES / 2;  // with phases: the half that is one behind
 
     // ---- this workgroup's sequence, kv head, tile of pairs and piece
     int b = 0, tile = 0, kvh = 0, piece = 0;
@@ -840,7 +853,6 @@ kv8_prefill_kernel(Kv8PrefillArgs a) {
 }
 
 // ------------------------------------------------------------- host side
-
 
 struct Kv8PrefillPlan {
     int chunk, waves, pieces;

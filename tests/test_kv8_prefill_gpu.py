@@ -288,6 +288,58 @@ def test_prefill_in_graphs(gpu):
             o.zero_()
 
 
+def test_a_captured_step_serves_other_batches(gpu):
+    """Map, write and attention captured once, for at most five sequences and 96 rows, replayed for batches of other
+    lengths, padded ones among them, against the same calls made eagerly."""
+    heads, q_heads, bt, dim, batch, n_rows, n_blocks = 2, 8, 16, 64, 5, 96, 64
+    i32 = lambda *s: torch.zeros(*s, dtype=torch.int32, device="cuda")  # noqa: E731
+
+    def state():
+        return dict(cache=gpu.Kv8Cache.empty(n_blocks, heads, bt, dim), cached=i32(batch), new=i32(batch),
+                    free=i32(n_blocks), tables=torch.full((batch, 20), -1, dtype=torch.int32, device="cuda"),
+                    ctx=i32(batch), starts=i32(batch + 1), slots=torch.zeros(n_rows, dtype=torch.int64, device="cuda"),
+                    positions=i32(n_rows), counts=i32(2), kv=torch.zeros(2, n_rows, heads, dim, device="cuda"),
+                    q=torch.zeros(n_rows, q_heads, dim, dtype=torch.bfloat16, device="cuda"),
+                    out=torch.zeros(n_rows, q_heads, dim, dtype=torch.bfloat16, device="cuda"),
+                    ws=gpu.alloc_workspace(1 << 24))
+
+    def step(s):
+        gpu.batch_map(s["cached"], s["new"], s["free"], s["tables"], bt, n_blocks, s["ctx"], s["starts"], s["slots"],
+                      s["positions"], s["counts"])
+        gpu.kv8_write(s["cache"], s["slots"], s["kv"][0], s["kv"][1])
+        gpu.kv8_prefill_bf16(s["cache"], s["q"], s["tables"], s["ctx"], s["starts"], s["out"], max_rows=90, max_ctx=300,
+                             workspace=s["ws"])
+
+    eager, graphed = state(), state()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(graphed)
+    rng, lens, left = np.random.default_rng(61), np.zeros(batch, np.int32), rng_blocks(n_blocks)
+    for new in ([40, 3, 0, 17, 0], [1, 1, 0, 1, 0], [1, 16, 60, 1, 1], [0, 0, 0, 0, 0], [90, 1, 1, 1, 3], [1, 1, 1, 1, 1]):
+        new = np.array(new, np.int32)
+        kv = torch.from_numpy(rng.standard_normal((2, n_rows, heads, dim)).astype(np.float32)).cuda()
+        q = torch.from_numpy(rng.standard_normal((n_rows, q_heads, dim)).astype(np.float32)).cuda().bfloat16()
+        for s in (eager, graphed):
+            s["cached"].copy_(dev(lens)), s["new"].copy_(dev(new)), s["kv"].copy_(kv), s["q"].copy_(q)
+            s["free"].fill_(-1)
+            s["free"][:len(left)].copy_(dev(left)), s["out"].fill_(-7.0)
+        step(eager)
+        graph.replay()
+        torch.cuda.synchronize()
+        for name in ("tables", "ctx", "starts", "slots", "positions", "counts", "out"):
+            assert torch.equal(eager[name], graphed[name]), name
+        for name in ("k", "v", "k_scales", "v_scales"):
+            assert torch.equal(getattr(eager["cache"], name), getattr(graphed["cache"], name)), name
+        lens, rows = lens + new, int(new.sum())
+        assert (eager["ctx"].cpu().numpy() == lens).all() and int(eager["counts"][1]) == rows
+        assert (eager["out"][rows:] == -7.0).all() and eager["out"][:rows].isfinite().all()
+        left = left[int(eager["counts"][0]):]
+
+
+def rng_blocks(n):
+    return np.random.default_rng(n).permutation(n).astype(np.int32)
+
+
 def test_prompts_then_decode(gpu):
     """A batch's prompts mapped, written and attended in one step, then a decode step on top of them."""
     rng = np.random.default_rng(31)
