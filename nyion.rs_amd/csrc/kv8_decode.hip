@@ -37,10 +37,9 @@
 // the order of the pieces, so that the order of arrival changes nothing.
 //
 // Bound: the cache's bytes at batch (64 sequences of 16640 tokens, 32/4 heads of
-// 64: 104 us, 5.25 TB/s, where the same kernel without its products takes 103;
-// 24 of 200-16000, 32/8 of 128: 87 us, 4.6 TB/s, with capped scores 96); for single
-// sequences the chain length -> table -> rows -> partials -> join (32 tokens to
-// 128: 4.7 us; 4096 of 4 kv heads of 64: 9.3 us; 32768: 15.5 us).
+// 64: 95.5 us, 5.7 TB/s; 24 of 200-16000, 32/8 of 128: 82.5 us, 4.8 TB/s, int8 with
+// capped scores 92); for single sequences the chain length -> table -> rows ->
+// partials -> join (4 kv heads of 64: 128 tokens 4.5 us, 4096 9.2, 32768 15.1).
 #include <limits.h>
 
 #include <algorithm>
@@ -147,7 +146,7 @@ __device__ __forceinline__ Kv8Span kv8_span(const Kv8DecodeArgs& a, int ctx) {
     return r;
 }
 
-template <int D, int CODE, bool MODS>
+template <int D, int CODE, bool MODS, bool PASSING>
 __global__ __launch_bounds__(64 * kWaves, 2) void kv8_decode_kernel(Kv8DecodeArgs a) {
     using Tile = Kv8Tile<D>;
     constexpr int KC = Tile::KC, VW = Tile::VW;
@@ -354,6 +353,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_decode_kernel(Kv8DecodeArg
             }
             absent = ~__ballot(present);
         };
+        const auto get = [](const auto* p) __attribute__((always_inline)) {
+            return PASSING ? __builtin_nontemporal_load(p) : *p;
+        };
         auto load = [&](Tile& t, int i) __attribute__((always_inline)) {
 #pragma unroll
             for (int u = 0; u < 4; u++) {
@@ -363,15 +365,15 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_decode_kernel(Kv8DecodeArg
                 const uint8_t* kb = a.c.k + at;
                 const uint8_t* vb = a.c.v + at;
 #pragma unroll
-                for (int c = 0; c < KC; c++) t.k[u][c] = *(const u32x4_t*)(kb + (klane + 64 * c));
+                for (int c = 0; c < KC; c++) t.k[u][c] = get((const u32x4_t*)(kb + (klane + 64 * c)));
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
                     if constexpr (VW == 2) {
-                        const u32x2_t w = *(const u32x2_t*)(vb + (vlane + 4 * D * r));
+                        const u32x2_t w = get((const u32x2_t*)(vb + (vlane + 4 * D * r)));
                         t.v[u][r][0] = w[0];
                         t.v[u][r][1] = w[1];
                     } else {
-                        t.v[u][r][0] = *(const uint32_t*)(vb + (vlane + 4 * D * r));
+                        t.v[u][r][0] = get((const uint32_t*)(vb + (vlane + 4 * D * r)));
                     }
                 }
             }
@@ -751,11 +753,19 @@ constexpr int kMinTiles = 4;
 // 25.4 / 21.1 / 21.1; three of 3000-9000, 32/8 of 128, 18.2 / 17.1 / 17.2.
 constexpr int kDirectSegments = 64;
 constexpr long long kMaxDirectPieces = 32;
+// Launches that may read more than the memory-side cache holds (256 MB, by the bound of
+// the lengths, each row once) read past it with nontemporal loads: their rows would be
+// gone from it before the next launch.  Measured (us, through it / past it): 64 sequences
+// of 16640 tokens, 32/4 heads of 64 (545 MB) 104 / 95.4, of 512-32768 111 / 102.5, 24 of
+// 200-16000, 32/8 of 128 (399 MB) 86.4 / 82.5; what fits finds itself there again: 64 of
+// 2048 (67 MB) 18.1 / 19.3, seven of 8000, 32/8 of 128 (115 MB) 19.2 / 23.0.
+constexpr long long kPassingBytes = 1LL << 28;
 
 struct Kv8DecodePlan {
     int units, chunk, pieces, grid;
     int slots;
     size_t acc, ml, bytes;
+    bool passing;
 };
 
 static int decode_plan(Kv8DecodePlan& p, const Kv8& c, int batch, int n_heads, int max_ctx, int window,
@@ -780,6 +790,7 @@ static int decode_plan(Kv8DecodePlan& p, const Kv8& c, int batch, int n_heads, i
         p.pieces = 0;
         p.grid = (int)std::min((long long)kMaxWgs, (tiles * segments + kMinTiles - 1) / kMinTiles);
     }
+    p.passing = segments > kDirectSegments && group <= 16 && segments * tiles * kTile * 2 * c.head_dim > kPassingBytes;
     p.slots = p.pieces ? p.grid : 2 * p.grid;
     const size_t slots = (size_t)p.slots;
     p.acc = slots * 16 * c.head_dim * sizeof(float);
@@ -788,14 +799,14 @@ static int decode_plan(Kv8DecodePlan& p, const Kv8& c, int batch, int n_heads, i
     return NYION_OK;
 }
 
-template <int D, int CODE, bool MODS>
+template <int D, int CODE, bool MODS, bool PASSING>
 static int resident_wgs() {
     static std::atomic<int> cache[kMaxDevices];
     return per_device_value(
         cache,
         [] {
             int per_cu = 0;
-            if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, kv8_decode_kernel<D, CODE, MODS>, 64 * kWaves,
+            if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, kv8_decode_kernel<D, CODE, MODS, PASSING>, 64 * kWaves,
                                                              0) != hipSuccess) {
                 (void)hipGetLastError();
                 return 0;
@@ -805,10 +816,10 @@ static int resident_wgs() {
         512);
 }
 
-template <int D, int CODE, bool MODS>
+template <int D, int CODE, bool MODS, bool PASSING>
 static void launch_decode(const Kv8DecodeArgs& a, int grid, hipStream_t stream) {
-    if (a.pieces == 0) grid = std::min(grid, resident_wgs<D, CODE, MODS>());
-    hipLaunchKernelGGL((kv8_decode_kernel<D, CODE, MODS>), dim3(grid), dim3(64 * kWaves), 0, stream, a);
+    if (a.pieces == 0) grid = std::min(grid, resident_wgs<D, CODE, MODS, PASSING>());
+    hipLaunchKernelGGL((kv8_decode_kernel<D, CODE, MODS, PASSING>), dim3(grid), dim3(64 * kWaves), 0, stream, a);
 }
 
 }  // namespace nyion
@@ -886,10 +897,14 @@ int nyion_kv8_decode_attention(const nyion_kv8_cache* cache, const int32_t* bloc
         a.out = (char*)out + b0 * row * size;
         auto by_mods = [&](auto d, auto code) {
             constexpr int D = decltype(d)::value, CODE = decltype(code)::value;
-            if (mods)
-                launch_decode<D, CODE, true>(a, p.grid, (hipStream_t)stream);
+            if (mods && p.passing)
+                launch_decode<D, CODE, true, true>(a, p.grid, (hipStream_t)stream);
+            else if (mods)
+                launch_decode<D, CODE, true, false>(a, p.grid, (hipStream_t)stream);
+            else if (p.passing)
+                launch_decode<D, CODE, false, true>(a, p.grid, (hipStream_t)stream);
             else
-                launch_decode<D, CODE, false>(a, p.grid, (hipStream_t)stream);
+                launch_decode<D, CODE, false, false>(a, p.grid, (hipStream_t)stream);
         };
         auto by_code = [&](auto d) {
             if (cache->code == NYION_KV8_E4M3)

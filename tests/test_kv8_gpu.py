@@ -391,6 +391,14 @@ def test_decode_does_not_depend_on_max_ctx(gpu):
         check_decode(gpu, E4M3, [900, 33] * 40, 8, 2, 16, 64, max_ctx=max_ctx)
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("code,options", [(E4M3, {}), (INT8, {}), (E4M3, dict(softcap=30.0)), (INT8, dict(softcap=30.0))])
+def test_decode_of_batches_that_may_be_large(gpu, code, options, dim):
+    """Bounds from which a launch reads past the memory-side cache."""
+    lens = np.random.default_rng(23).integers(0, 700, 40).tolist()
+    check_decode(gpu, code, lens, 8, 2, 32, dim, max_ctx=1 << 20, **options)
+
+
 def test_decode_skips_pages_that_are_no_blocks(gpu):
     """Entries past the cache or negative, at a tile's edge and inside it, in the middle and at the end."""
     for drop in ([(1, -1)], [(0, 2 ** 31 - 1), (5, -7)], [(4, 10 ** 6), (5, -1), (6, -1), (7, -1)],
