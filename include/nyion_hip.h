@@ -714,12 +714,12 @@ int nyion_kv8_decode_attention(const nyion_kv8_cache* cache, const int32_t* bloc
  * row r at position ctx_lens[b] - row_starts[b + 1] + r; their K/V are in the
  * cache already.  Rows behind row_starts[batch] are left as they are in out,
  * rows of row_starts behind n_rows are not computed, and rows at negative
- * positions give zeros.  max_rows and max_ctx, bounds of
- * the rows and the length of one sequence, shape the launch and the
- * workspace, not the result.  q is carried exactly (bf16 relative to the
- * row's largest value in binary16), weights and V in binary16 (11 bits), sums
- * in f32; n_rows * n_heads at most 2^27.  Everything else as for
- * nyion_kv8_decode_attention. */
+ * positions give zeros.  max_rows and max_ctx, bounds of the rows and the
+ * length of one sequence, shape the launch and the workspace, not the result
+ * (rows of a sequence past max_rows may be left as they are in out).  q is
+ * carried exactly (bf16 relative to the row's largest value in binary16),
+ * weights and V in binary16 (11 bits) or better, sums in f32; n_rows * n_heads
+ * at most 2^27.  Everything else as for nyion_kv8_decode_attention. */
 size_t nyion_kv8_prefill_workspace_size(const nyion_kv8_cache* cache, int batch, int n_heads,
                                         int n_rows, int max_rows, int max_ctx, int window);
 int nyion_kv8_prefill_attention_bf16(const nyion_kv8_cache* cache, const int32_t* block_tables,

@@ -40,6 +40,30 @@ int kv8_cache_args(Kv8& c, const nyion_kv8_cache* cache, const char* what);
 int kv8_score_args(ScoreArgs& s, const nyion_score_options* o, int head_dim, bool prefix_ok,
                    const char* what);
 
+// A ragged batch of few rows a sequence, as the decode takes it from the prefill
+// (kv8_decode.hip): q and out bf16.
+struct Kv8FewRows {
+    Kv8 c;
+    ScoreArgs s;
+    int code;
+    const int32_t* tables;
+    int max_blocks;
+    const int32_t* ctx_lens;
+    const int32_t* row_starts;
+    int batch, n_rows, max_rows, max_ctx;
+    const uint16_t* q;
+    long long q_stride;
+    uint16_t* out;
+    int n_heads;
+    void* workspace;
+    size_t workspace_bytes;
+    hipStream_t stream;
+};
+bool kv8_few_rows(const Kv8& c, int batch, int n_heads, int n_rows, int max_rows);
+int kv8_few_rows_size(size_t& bytes, const Kv8& c, int batch, int n_heads, int max_rows, int max_ctx, int window,
+                      const char* what);
+int kv8_few_rows_attention(const Kv8FewRows& x, const char* what);
+
 // Token t's block in a sequence's table, or -1: past the table (or t
 // negative), or not a block of the cache.
 __device__ __forceinline__ int kv8_block(const Kv8& c, const int32_t* table, int max_blocks, int t) {

@@ -1,7 +1,8 @@
 // kv8_decode.hip — batched decode attention over the 8-bit cache (gfx950).
 //
-// One query row per sequence.  A segment is one (sequence, kv head, group of
-// up to 16 q heads); its keys are cut into tiles of 64 positions, four
+// One query row per sequence (or few, which the prefill hands over: their (row,
+// head) pairs then stand in for heads).  A segment is one (sequence, kv head,
+// group of up to 16 q heads); its keys are cut into tiles of 64 positions, four
 // subtiles of 16, each inside one cache block and so with one K and one V
 // scale.  Per tile a wavefront computes, on v_mfma_f32_16x16x32_f16,
 //   S^T[16 tokens][16 heads] += K . Q^T     per subtile, K codes as binary16
@@ -72,11 +73,13 @@ struct Kv8DecodeArgs {
     int batch;
     int n_heads;
     int group;       // q heads per kv head
-    int n_hg;        // head groups of 16 per kv head
+    int n_hg;        // groups of 16 heads, or (row, head) pairs, per kv head
     int pieces;      // > 0: each segment is cut into up to this many pieces
     int min_tiles;   // fewest tiles of a workgroup
     int slots;       // partials that the workspace holds
     int bf16;
+    int n_rows;      // with several rows per sequence only
+    const int32_t* row_starts;
 };
 
 // max(v, v of lane ^ 16), then ^ 32: the lanes of one head
@@ -146,7 +149,35 @@ __device__ __forceinline__ Kv8Span kv8_span(const Kv8DecodeArgs& a, int ctx) {
     return r;
 }
 
-template <int D, int CODE, bool MODS, bool PASSING>
+// The same for a sequence of several rows: the keys that any of them sees.
+struct Kv8Rows {
+    int row0, rows, pos0, live, prefix;
+};
+__device__ __forceinline__ Kv8Rows kv8_rows(const Kv8DecodeArgs& a, int b) {
+    Kv8Rows s;
+    const int end = a.row_starts[b + 1], ctx = a.ctx_lens[b];
+    s.row0 = min(max(a.row_starts[b], 0), a.n_rows);
+    s.rows = min(max(end, s.row0), a.n_rows) - s.row0;
+    s.pos0 = (int)((unsigned)ctx - (unsigned)end + (unsigned)s.row0);
+    s.live = max(min(ctx, a.span), 0);
+    s.prefix = a.s.prefix_lens ? a.s.prefix_lens[b] : 0;
+    return s;
+}
+__device__ __forceinline__ int key_end(const Kv8Rows& s, int pos) {
+    return pos < 0 ? 0 : min(max(pos + 1, s.prefix), s.live);
+}
+__device__ __forceinline__ Kv8Span kv8_span(const Kv8DecodeArgs& a, const Kv8Rows& s) {
+    Kv8Span r;
+    r.hi = s.rows > 0 ? key_end(s, s.pos0 + s.rows - 1) : 0;
+    r.lo = a.s.window > 0 ? min(max(s.pos0 - a.s.window + 1, 0), r.hi) : 0;
+    r.first = r.lo / kTile;
+    r.tiles = max((int)(((unsigned)r.hi + kTile - 1) / kTile) - r.first, 1);
+    return r;
+}
+
+// ROWS: several rows per sequence, as few as the prefill hands over: a segment is 16
+// (row, head) pairs of a kv head, numbered row-major.
+template <int D, int CODE, bool MODS, bool PASSING, bool ROWS>
 __global__ __launch_bounds__(64 * kWaves, 2) void kv8_decode_kernel(Kv8DecodeArgs a) {
     using Tile = Kv8Tile<D>;
     constexpr int KC = Tile::KC, VW = Tile::VW;
@@ -167,6 +198,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_decode_kernel(Kv8DecodeArg
     const int n = lane & 15;   // head of the group / row of an A operand
     const int g = lane >> 4;   // lane group
     const int units = a.c.n_kv_heads * a.n_hg;
+    const auto span_of = [&](int b, int ctx) {
+        if constexpr (ROWS)
+            return kv8_span(a, kv8_rows(a, b));
+        else
+            return kv8_span(a, ctx);
+    };
 
     // Where this workgroup's tiles lie: of `total` tiles each of `wgs`
     // workgroups takes total / wgs, the first total % wgs one more.
@@ -176,7 +213,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_decode_kernel(Kv8DecodeArg
         uint32_t total;
         if (a.batch <= 64) {
             seq_ctx = lane < a.batch ? a.ctx_lens[lane] : 0;
-            seq_end = lane < a.batch ? kv8_span(a, seq_ctx).tiles : 0;
+            seq_end = lane < a.batch ? span_of(lane, seq_ctx).tiles : 0;
 #pragma unroll
             for (int d = 1; d < 64; d <<= 1) {
                 const int y = __shfl_up(seq_end, d);
@@ -187,7 +224,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_decode_kernel(Kv8DecodeArg
             int before = 0;
             for (int b0 = 0; b0 < a.batch; b0 += 64 * kWaves) {
                 const int b = b0 + tid;
-                int x = b < a.batch ? kv8_span(a, a.ctx_lens[b]).tiles : 0;
+                int x = b < a.batch ? span_of(b, a.ctx_lens[b]).tiles : 0;
 #pragma unroll
                 for (int d = 1; d < 64; d <<= 1) {
                     const int y = __shfl_up(x, d);
@@ -226,10 +263,18 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_decode_kernel(Kv8DecodeArg
     constexpr int DPT = D / 16;
     const int row = tid >> 4;
     const int d0 = (tid & 15) * DPT;
+    // b: the sequence's (first) row of out; head0: the segment's first head, with
+    // several rows per sequence its unit
     const auto write_out = [&](const float (&o)[DPT], float ol, int b, int head0, int heads) __attribute__((always_inline)) {
         if (row >= heads) return;
         const float inv = ol == 0.f ? 0.f : 1.f / ol;  // nothing seen: zeros
-        const long long at = ((long long)b * a.n_heads + head0 + row) * D + d0;
+        long long at;
+        if constexpr (ROWS) {
+            const int kvh = head0 / a.n_hg, x = (head0 - kvh * a.n_hg) * 16 + row, i = x / a.group;
+            at = ((long long)(b + i) * a.n_heads + kvh * a.group + (x - i * a.group)) * D + d0;
+        } else {
+            at = ((long long)b * a.n_heads + head0 + row) * D + d0;
+        }
         if (a.bf16) {
 #pragma unroll
             for (int e = 0; e < DPT; e += 4) {
@@ -260,7 +305,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_decode_kernel(Kv8DecodeArg
             const int p = (int)blockIdx.x - seg * a.pieces;
             b = seg / units;
             ctx = __builtin_amdgcn_readfirstlane(a.ctx_lens[b]);
-            sp = kv8_span(a, ctx);
+            sp = span_of(b, ctx);
             n_pieces = min(a.pieces, (sp.tiles + a.min_tiles - 1) / a.min_tiles);
             if (p >= n_pieces) return;
             // pieces of tiles / n_pieces, the first ones one more
@@ -289,7 +334,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_decode_kernel(Kv8DecodeArg
                 before = b > 0 ? __builtin_amdgcn_readfirstlane(sm_ends[b - 1]) : 0;
                 ctx = __builtin_amdgcn_readfirstlane(a.ctx_lens[b]);
             }
-            sp = kv8_span(a, ctx);
+            sp = span_of(b, ctx);
             const uint32_t seq0 = (uint32_t)before * units;
             const uint32_t unit = (pos - seq0) / (uint32_t)sp.tiles;
             const uint32_t start = seq0 + unit * sp.tiles;  // of the segment
@@ -310,13 +355,30 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_decode_kernel(Kv8DecodeArg
         const int unit = seg - b * units;
         const int kvh = unit / a.n_hg;
         const int hg = unit - kvh * a.n_hg;
-        const int head0 = kvh * a.group + hg * 16;
-        const int heads = min(16, a.group - hg * 16);
         const int32_t* table = a.tables + (long long)b * a.max_blocks;
-        const int qpos = ctx - 1;
+        const int head0 = kvh * a.group + (ROWS ? 0 : hg * 16);
+        int heads = min(16, a.group - hg * 16);
+        int qpos = ctx - 1;
+        int row0 = 0, i = 0, mine = n;  // ROWS: the sequence's first row, this lane's of it, its head of the group
+        int key_lo, key_hi, all_lo, all_hi;  // ROWS: what this lane's pair sees, what all pairs see
+        if constexpr (ROWS) {
+            const Kv8Rows rows = kv8_rows(a, b);
+            const int x0 = hg * 16;
+            row0 = rows.row0;
+            heads = max(min(16, rows.rows * a.group - x0), 0);
+            const int last = max(heads - 1, 0), x = x0 + min(n, last);
+            i = x / a.group;
+            mine = x - i * a.group;
+            const int first_pos = rows.pos0 + x0 / a.group, last_pos = rows.pos0 + (x0 + last) / a.group;
+            qpos = rows.pos0 + i;
+            key_hi = key_end(rows, qpos);
+            all_hi = key_end(rows, first_pos);
+            key_lo = a.s.window > 0 ? max(qpos - a.s.window + 1, 0) : 0;
+            all_lo = a.s.window > 0 ? max(last_pos - a.s.window + 1, 0) : 0;
+        }
 
         float slope = 0.f;
-        if (MODS && a.s.slopes && n < heads) slope = a.s.slopes[head0 + n] * 1.4426950408889634f;
+        if (MODS && a.s.slopes && n < heads) slope = a.s.slopes[head0 + mine] * 1.4426950408889634f;
 
         float4_t acc[MT];
 #pragma unroll
@@ -328,6 +390,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_decode_kernel(Kv8DecodeArg
         const int tn = t1 - t0;
         const int tw0 = sp.first + t0 + tn * wave / kWaves;
         int te = sp.first + t0 + tn * (wave + 1) / kWaves;
+        if (ROWS && heads == 0) te = tw0;  // pairs that this sequence does not have
 
         const uint32_t klane = (uint32_t)((4 * (n & 3) + (n >> 2)) * D + 16 * g);
         const uint32_t vlane = (uint32_t)(g * D + 4 * VW * n);
@@ -387,7 +450,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_decode_kernel(Kv8DecodeArg
         float xq[2 * KC][8];
 #pragma unroll
         for (int c = 0; c < 2 * KC; c++) {
-            const long long at = b * a.q_stride + (long long)(head0 + n) * D + 64 * (c >> 1) + 16 * g + 8 * (c & 1);
+            const long long at =
+                (ROWS ? row0 + i : b) * a.q_stride + (long long)(head0 + mine) * D + 64 * (c >> 1) + 16 * g + 8 * (c & 1);
             if (n >= heads) {
 #pragma unroll
                 for (int e = 0; e < 8; e++) xq[c][e] = 0.f;
@@ -445,7 +509,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_decode_kernel(Kv8DecodeArg
             auto use = [&](Tile& t, int i) __attribute__((always_inline)) {
                 const int p0 = (tb + i) * kTile;
                 const int gone = (int)(absent >> (4 * i)) & 15;
-                const bool masked = p0 < sp.lo || p0 > sp.hi - kTile || gone;
+                const bool masked = ROWS ? p0 < all_lo || p0 > all_hi - kTile || gone
+                                         : p0 < sp.lo || p0 > sp.hi - kTile || gone;
                 // two subtiles' chains side by side: a chain's MFMAs wait for each other
                 float4_t s[4];
 #pragma unroll
@@ -500,7 +565,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_decode_kernel(Kv8DecodeArg
                         for (int u = 0; u < 4; u++)
 #pragma unroll
                             for (int r = 0; r < 4; r++)
-                                s[u][r] = __builtin_fmaf(-slope, back - (float)(16 * u + 4 * r), s[u][r]);
+                                s[u][r] = __builtin_fmaf(-slope,
+                                                         ROWS ? fabsf(back - (float)(16 * u + 4 * r))
+                                                              : back - (float)(16 * u + 4 * r),
+                                                         s[u][r]);
                     }
                 }
                 if (masked) {
@@ -510,10 +578,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_decode_kernel(Kv8DecodeArg
 #pragma unroll
                         for (int r = 0; r < 4; r++) {
                             const int key = p0 + 16 * u + 4 * r + g;
-                            const bool seen = key >= sp.lo && key < sp.hi && !((gone >> u) & 1);
+                            const bool held = key >= sp.lo && key < sp.hi && !((gone >> u) & 1);
+                            bool seen = held;
+                            if constexpr (ROWS) seen = held && key >= key_lo && key < key_hi;
                             s[u][r] = seen ? s[u][r] * f[u] : -INFINITY;
 #pragma unroll
-                            for (int x = 0; x < VW; x++) t.v[u][r][x] = seen ? t.v[u][r][x] : 0u;
+                            for (int x = 0; x < VW; x++) t.v[u][r][x] = held ? t.v[u][r][x] : 0u;
                         }
                         f[u] = 1.f;
                     }
@@ -626,7 +696,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_decode_kernel(Kv8DecodeArg
             for (int e = 0; e < DPT; e++) o[e] = __builtin_fmaf(sm_acc[w][row][d0 + e], f, o[e]);
         }
         if (n_pieces == 1) {
-            write_out(o, ol, b, head0, heads);
+            write_out(o, ol, ROWS ? row0 : b, ROWS ? unit : head0, heads);
         } else {
             if (row < heads) {
                 const int mine = slot_mine * 16 + row;
@@ -640,7 +710,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_decode_kernel(Kv8DecodeArg
                     __builtin_amdgcn_raw_buffer_store_b64(u32x2_t{__float_as_uint(om), __float_as_uint(ol)}, rml,
                                                           mine * 8, 0, kSc1);
             }
-            if (tid == 0) sm_shared[n_shared] = {n_pieces, slot0, slot1, b, head0, heads};
+            if (tid == 0) sm_shared[n_shared] = {n_pieces, slot0, slot1, ROWS ? row0 : b, ROWS ? unit : head0, heads};
             n_shared++;
         }
         if (a.pieces > 0) break;
@@ -672,6 +742,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_decode_kernel(Kv8DecodeArg
         const int heads = sh.heads, n_pieces = sh.n_pieces;
         // 16 threads a head; what is left of the workgroup takes every
         // `groups`-th piece, so that one round of loads has many
+        if (ROWS && heads == 0) {  // nothing to join
+            if (tid == 0) __hip_atomic_store(a.counters + sh.slot0, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            continue;
+        }
         const int rows = heads > 8 ? 16 : heads > 4 ? 8 : heads > 2 ? 4 : heads;  // a power of two
         const int groups = 16 / rows;
         const int mrow = row & (rows - 1), mgrp = row / rows;
@@ -760,6 +834,15 @@ constexpr long long kMaxDirectPieces = 32;
 // 200-16000, 32/8 of 128 (399 MB) 86.4 / 82.5; what fits finds itself there again: 64 of
 // 2048 (67 MB) 18.1 / 19.3, seven of 8000, 32/8 of 128 (115 MB) 19.2 / 23.0.
 constexpr long long kPassingBytes = 1LL << 28;
+// Rows that the prefill hands over: up to 16 (row, head) pairs of a kv head, one segment
+// per sequence and kv head, or up to 64 in launches of few segments, whose time is the
+// chain's and not that of reading the keys once for every 16 pairs.  Measured (us, the
+// prefill's kernel / here; 32/8 heads of 128 behind 2000 tokens, batch x rows): 1 x 4
+// behind 30000 59.5 / 27.7, 64 x 4 (16 pairs) 93 / 56; 1 x 16 behind 16000 (64 pairs, 32
+// segments) 41.1 / 25.2, 4 x 16 (128 segments) 22.0 / 20.6, 16 x 8 (256) 39.1 / 31.4, 8 x 16
+// (256) 30.1 / 31.2, 64 x 16 (2048) 95 / 169.
+constexpr int kFewPairs = 64;
+constexpr int kFewSegments = 256;
 
 struct Kv8DecodePlan {
     int units, chunk, pieces, grid;
@@ -769,7 +852,7 @@ struct Kv8DecodePlan {
 };
 
 static int decode_plan(Kv8DecodePlan& p, const Kv8& c, int batch, int n_heads, int max_ctx, int window,
-                       const char* what) {
+                       int max_rows, const char* what) {
     if (batch <= 0 || n_heads <= 0 || max_ctx <= 0)
         return set_error(NYION_ERR_INVALID, "%s: batch, n_heads and max_ctx must be positive", what);
     if (n_heads % c.n_kv_heads)
@@ -777,10 +860,11 @@ static int decode_plan(Kv8DecodePlan& p, const Kv8& c, int batch, int n_heads, i
                          c.n_kv_heads);
     if (n_heads > 16384) return set_error(NYION_ERR_UNSUPPORTED, "%s: n_heads %d", what, n_heads);
     const int group = n_heads / c.n_kv_heads;
-    p.units = c.n_kv_heads * ((group + 15) / 16);
+    p.units = c.n_kv_heads * ((max_rows * group + 15) / 16);
     p.chunk = std::min(batch, kMaxSeqs);
     const long long segments = (long long)p.chunk * p.units;
-    const long long keys = window > 0 ? std::min((long long)window + kTile, (long long)max_ctx) : max_ctx;
+    const long long keys =
+        window > 0 ? std::min((long long)window + max_rows + kTile, (long long)max_ctx) : max_ctx;
     const long long tiles = (keys + kTile - 1) / kTile;
     if (segments <= kDirectSegments) {
         const long long fill = std::min(std::max(device_cu_count() / segments, 1LL), kMaxDirectPieces);
@@ -790,7 +874,7 @@ static int decode_plan(Kv8DecodePlan& p, const Kv8& c, int batch, int n_heads, i
         p.pieces = 0;
         p.grid = (int)std::min((long long)kMaxWgs, (tiles * segments + kMinTiles - 1) / kMinTiles);
     }
-    p.passing = segments > kDirectSegments && group <= 16 && segments * tiles * kTile * 2 * c.head_dim > kPassingBytes;
+    p.passing = max_rows == 1 && segments > kDirectSegments && group <= 16 && segments * tiles * kTile * 2 * c.head_dim > kPassingBytes;
     p.slots = p.pieces ? p.grid : 2 * p.grid;
     const size_t slots = (size_t)p.slots;
     p.acc = slots * 16 * c.head_dim * sizeof(float);
@@ -799,27 +883,130 @@ static int decode_plan(Kv8DecodePlan& p, const Kv8& c, int batch, int n_heads, i
     return NYION_OK;
 }
 
-template <int D, int CODE, bool MODS, bool PASSING>
+template <int D, int CODE, bool MODS, bool PASSING, bool ROWS>
 static int resident_wgs() {
     static std::atomic<int> cache[kMaxDevices];
     return per_device_value(
         cache,
         [] {
             int per_cu = 0;
-            if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, kv8_decode_kernel<D, CODE, MODS, PASSING>, 64 * kWaves,
+            if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, kv8_decode_kernel<D, CODE, MODS, PASSING, ROWS>, 64 * kWaves,
                                                              0) != hipSuccess) {
                 (void)hipGetLastError();
                 return 0;
             }
-            return std::max(per_cu, 1) * device_cu_count();
+            // more than two measured slower (64 sequences of 2048 tokens 18.1 / 22.3 us)
+            return std::min(std::max(per_cu, 1), 2) * device_cu_count();
         },
         512);
 }
 
-template <int D, int CODE, bool MODS, bool PASSING>
+template <int D, int CODE, bool MODS, bool PASSING, bool ROWS>
 static void launch_decode(const Kv8DecodeArgs& a, int grid, hipStream_t stream) {
-    if (a.pieces == 0) grid = std::min(grid, resident_wgs<D, CODE, MODS, PASSING>());
-    hipLaunchKernelGGL((kv8_decode_kernel<D, CODE, MODS, PASSING>), dim3(grid), dim3(64 * kWaves), 0, stream, a);
+    if (a.pieces == 0) grid = std::min(grid, resident_wgs<D, CODE, MODS, PASSING, ROWS>());
+    hipLaunchKernelGGL((kv8_decode_kernel<D, CODE, MODS, PASSING, ROWS>), dim3(grid), dim3(64 * kWaves), 0, stream, a);
+}
+
+// Launches of up to p.chunk sequences each; what a.q, a.out and the lists point to is the
+// first sequence's.
+static int launch_chunks(Kv8DecodeArgs a, const Kv8DecodePlan& p, int code, int batch, void* d_workspace,
+                         size_t workspace_bytes, hipStream_t stream, const char* what) {
+    if (p.bytes) {
+        if (!d_workspace || workspace_bytes < p.bytes)
+            return set_error(NYION_ERR_WORKSPACE, "%s: workspace %zu bytes < required %zu", what,
+                             d_workspace ? workspace_bytes : (size_t)0, p.bytes);
+        if (!aligned(d_workspace, 256))
+            return set_error(NYION_ERR_INVALID, "%s: workspace not 256-byte aligned", what);
+    }
+    a.counters = (int*)d_workspace;
+    a.ws_acc = (float*)((char*)d_workspace + kKv8CounterBytes);
+    a.ws_ml = (float2*)((char*)a.ws_acc + p.acc);
+    a.group = a.n_heads / a.c.n_kv_heads;
+    a.n_hg = p.units / a.c.n_kv_heads;
+    a.pieces = p.pieces;
+    a.min_tiles = kMinTiles;
+    a.slots = p.slots;
+    a.span = (int)std::min((long long)a.max_blocks << a.c.bt_log2, (long long)INT_MAX - 2 * kTile);
+    const bool mods = a.s.cap_log2 > 0.f || a.s.slopes, rows = a.row_starts != nullptr;
+    const int64_t size = a.bf16 ? 2 : 4;
+    int chunk = p.chunk;
+    if (!p.pieces) {  // a launch numbers its tiles in 32 bits
+        const long long per_seq = (long long)p.units * (a.span / kTile + 2);
+        chunk = (int)std::min((long long)chunk, (long long)INT_MAX / per_seq);
+        if (chunk < 1) return set_error(NYION_ERR_UNSUPPORTED, "%s: %lld tiles per sequence", what, per_seq);
+    }
+    for (int b0 = 0; b0 < batch; b0 += chunk) {
+        a.batch = std::min(chunk, batch - b0);
+        auto pick = [&](auto d, auto code) {
+            constexpr int D = decltype(d)::value, CODE = decltype(code)::value;
+            if (rows)
+                launch_decode<D, CODE, true, false, true>(a, p.grid, stream);
+            else if (mods && p.passing)
+                launch_decode<D, CODE, true, true, false>(a, p.grid, stream);
+            else if (mods)
+                launch_decode<D, CODE, true, false, false>(a, p.grid, stream);
+            else if (p.passing)
+                launch_decode<D, CODE, false, true, false>(a, p.grid, stream);
+            else
+                launch_decode<D, CODE, false, false, false>(a, p.grid, stream);
+        };
+        auto by_code = [&](auto d) {
+            if (code == NYION_KV8_E4M3)
+                pick(d, std::integral_constant<int, NYION_KV8_E4M3>{});
+            else
+                pick(d, std::integral_constant<int, NYION_KV8_INT8>{});
+        };
+        if (a.c.head_dim == 64)
+            by_code(std::integral_constant<int, 64>{});
+        else
+            by_code(std::integral_constant<int, 128>{});
+        int rc;
+        if ((rc = check_launch(what)) != NYION_OK) return rc;
+        a.tables += (int64_t)a.batch * a.max_blocks;
+        a.ctx_lens += a.batch;
+        if (rows) {
+            a.row_starts += a.batch;
+            if (a.s.prefix_lens) a.s.prefix_lens += a.batch;
+        } else {
+            a.q = (const char*)a.q + a.batch * a.q_stride * size;
+            a.out = (char*)a.out + (int64_t)a.batch * a.n_heads * a.c.head_dim * size;
+        }
+    }
+    return NYION_OK;
+}
+
+bool kv8_few_rows(const Kv8& c, int batch, int n_heads, int n_rows, int max_rows) {
+    const long long pairs = (long long)max_rows * (n_heads / c.n_kv_heads), sets = (pairs + 15) / 16;
+    return n_heads <= 16384 && n_rows <= (long long)batch * max_rows &&
+           (sets == 1 || (pairs <= kFewPairs && sets * batch * c.n_kv_heads <= kFewSegments));
+}
+
+int kv8_few_rows_size(size_t& bytes, const Kv8& c, int batch, int n_heads, int max_rows, int max_ctx, int window,
+                      const char* what) {
+    Kv8DecodePlan p;
+    const int rc = decode_plan(p, c, batch, n_heads, max_ctx, window, max_rows, what);
+    bytes = p.bytes;
+    return rc;
+}
+
+int kv8_few_rows_attention(const Kv8FewRows& x, const char* what) {
+    Kv8DecodeArgs a = {};
+    Kv8DecodePlan p;
+    int rc;
+    if ((rc = decode_plan(p, x.c, x.batch, x.n_heads, x.max_ctx, x.s.window, x.max_rows, what)) != NYION_OK) return rc;
+    a.c = x.c;
+    a.s = x.s;
+    a.tables = x.tables;
+    a.max_blocks = x.max_blocks;
+    a.ctx_lens = x.ctx_lens;
+    a.row_starts = x.row_starts;
+    a.n_rows = x.n_rows;
+    a.q = x.q;
+    a.out = x.out;
+    a.q_stride = x.q_stride;
+    a.n_heads = x.n_heads;
+    a.bf16 = 1;
+    return launch_chunks(a, p, x.code, x.batch, x.workspace, x.workspace_bytes, x.stream, what);
 }
 
 }  // namespace nyion
@@ -834,7 +1021,7 @@ size_t nyion_kv8_decode_workspace_size(const nyion_kv8_cache* cache, int batch, 
     Kv8 c;
     Kv8DecodePlan p;
     if (kv8_cache_args(c, cache, "kv8_decode_workspace_size") != NYION_OK ||
-        decode_plan(p, c, batch, n_heads, max_ctx, window, "kv8_decode_workspace_size") != NYION_OK)
+        decode_plan(p, c, batch, n_heads, max_ctx, window, 1, "kv8_decode_workspace_size") != NYION_OK)
         return 0;
     return p.bytes;
 }
@@ -848,11 +1035,11 @@ int nyion_kv8_decode_attention(const nyion_kv8_cache* cache, const int32_t* bloc
     int rc;
     if ((rc = require_device()) != NYION_OK) return rc;
     const char* what = "kv8_decode";
-    Kv8DecodeArgs a;
+    Kv8DecodeArgs a = {};
     Kv8DecodePlan p;
     if ((rc = kv8_cache_args(a.c, cache, what)) != NYION_OK) return rc;
     if ((rc = kv8_score_args(a.s, options, a.c.head_dim, false, what)) != NYION_OK) return rc;
-    if ((rc = decode_plan(p, a.c, batch, n_heads, max_ctx, a.s.window, what)) != NYION_OK) return rc;
+    if ((rc = decode_plan(p, a.c, batch, n_heads, max_ctx, a.s.window, 1, what)) != NYION_OK) return rc;
     if (io_dtype != NYION_IO_F32 && io_dtype != NYION_IO_BF16)
         return set_error(NYION_ERR_INVALID, "%s: io_dtype %d", what, io_dtype);
     if (!block_tables || !ctx_lens || !q || !out || max_blocks_per_seq <= 0)
@@ -862,63 +1049,15 @@ int nyion_kv8_decode_attention(const nyion_kv8_cache* cache, const int32_t* bloc
         return set_error(NYION_ERR_INVALID, "%s: q_stride %lld below n_heads * head_dim", what, (long long)q_stride);
     if (!aligned(q, 16) || !aligned(out, 16) || q_stride * size % 16)
         return set_error(NYION_ERR_INVALID, "%s: rows of q and out must be 16-byte aligned", what);
-    if (p.bytes) {
-        if (!d_workspace || workspace_bytes < p.bytes)
-            return set_error(NYION_ERR_WORKSPACE, "%s: workspace %zu bytes < required %zu", what,
-                             d_workspace ? workspace_bytes : (size_t)0, p.bytes);
-        if (!aligned(d_workspace, 256))
-            return set_error(NYION_ERR_INVALID, "%s: workspace not 256-byte aligned", what);
-    }
-    a.counters = (int*)d_workspace;
-    a.ws_acc = (float*)((char*)d_workspace + kKv8CounterBytes);
-    a.ws_ml = (float2*)((char*)a.ws_acc + p.acc);
-    a.q_stride = q_stride;
+    a.tables = block_tables;
     a.max_blocks = max_blocks_per_seq;
-    a.span = (int)std::min((long long)max_blocks_per_seq << a.c.bt_log2, (long long)INT_MAX - 2 * kTile);
+    a.ctx_lens = ctx_lens;
+    a.q = q;
+    a.out = out;
+    a.q_stride = q_stride;
     a.n_heads = n_heads;
-    a.group = n_heads / a.c.n_kv_heads;
-    a.n_hg = (a.group + 15) / 16;
-    a.pieces = p.pieces;
-    a.min_tiles = kMinTiles;
-    a.slots = p.slots;
     a.bf16 = io_dtype == NYION_IO_BF16;
-    const bool mods = a.s.cap_log2 > 0.f || a.s.slopes;
-    int chunk = p.chunk;
-    if (!p.pieces) {  // a launch numbers its tiles in 32 bits
-        const long long per_seq = (long long)p.units * (a.span / kTile + 2);
-        chunk = (int)std::min((long long)chunk, (long long)INT_MAX / per_seq);
-        if (chunk < 1) return set_error(NYION_ERR_UNSUPPORTED, "%s: %lld tiles per sequence", what, per_seq);
-    }
-    for (int b0 = 0; b0 < batch; b0 += chunk) {
-        a.batch = std::min(chunk, batch - b0);
-        a.tables = block_tables + (int64_t)b0 * max_blocks_per_seq;
-        a.ctx_lens = ctx_lens + b0;
-        a.q = (const char*)q + b0 * q_stride * size;
-        a.out = (char*)out + b0 * row * size;
-        auto by_mods = [&](auto d, auto code) {
-            constexpr int D = decltype(d)::value, CODE = decltype(code)::value;
-            if (mods && p.passing)
-                launch_decode<D, CODE, true, true>(a, p.grid, (hipStream_t)stream);
-            else if (mods)
-                launch_decode<D, CODE, true, false>(a, p.grid, (hipStream_t)stream);
-            else if (p.passing)
-                launch_decode<D, CODE, false, true>(a, p.grid, (hipStream_t)stream);
-            else
-                launch_decode<D, CODE, false, false>(a, p.grid, (hipStream_t)stream);
-        };
-        auto by_code = [&](auto d) {
-            if (cache->code == NYION_KV8_E4M3)
-                by_mods(d, std::integral_constant<int, NYION_KV8_E4M3>{});
-            else
-                by_mods(d, std::integral_constant<int, NYION_KV8_INT8>{});
-        };
-        if (a.c.head_dim == 64)
-            by_code(std::integral_constant<int, 64>{});
-        else
-            by_code(std::integral_constant<int, 128>{});
-        if ((rc = check_launch(what)) != NYION_OK) return rc;
-    }
-    return NYION_OK;
+    return launch_chunks(a, p, cache->code, batch, d_workspace, workspace_bytes, (hipStream_t)stream, what);
 }
 
 }  // extern "C"

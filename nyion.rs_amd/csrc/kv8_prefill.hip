@@ -32,7 +32,9 @@
 // of 32 weights passes 2^14; q is binary16 relative to its row's largest value.
 //
 // Few tiles: their keys are cut into pieces as well, joined through the
-// workspace by the last piece to arrive, in the order of the pieces.
+// workspace by the last piece to arrive, in the order of the pieces.  Few rows a
+// sequence (up to 16 pairs of a kv head, 64 in small launches): the decode's kernel
+// takes them (kv8_few_rows).
 //
 // Bound: the matrix unit and the power that it may draw for large launches
 // (8192 rows of 32/8 heads of 128: 534-565 us, 0.97-1.03 PFLOP/s, where a large
@@ -930,6 +932,10 @@ size_t nyion_kv8_prefill_workspace_size(const nyion_kv8_cache* cache, int batch,
     if (kv8_cache_args(c, cache, what) != NYION_OK ||
         prefill_plan(p, c, batch, n_heads, n_rows, max_rows, max_ctx, window, what) != NYION_OK)
         return 0;
+    if (kv8_few_rows(c, batch, n_heads, n_rows, max_rows)) {
+        size_t bytes;
+        return kv8_few_rows_size(bytes, c, batch, n_heads, max_rows, max_ctx, window, what) == NYION_OK ? bytes : 0;
+    }
     return p.bytes;
 }
 
@@ -957,6 +963,11 @@ int nyion_kv8_prefill_attention_bf16(const nyion_kv8_cache* cache, const int32_t
         return set_error(NYION_ERR_INVALID, "%s: q_stride %lld below n_heads * head_dim", what, (long long)q_stride);
     if (!aligned(q, 16) || !aligned(out, 16) || q_stride % 8)
         return set_error(NYION_ERR_INVALID, "%s: rows of q and out must be 16-byte aligned", what);
+    if (kv8_few_rows(a.c, batch, n_heads, n_rows, max_rows))
+        return kv8_few_rows_attention({a.c, a.s, cache->code, block_tables, max_blocks_per_seq, ctx_lens, row_starts,
+                                       batch, n_rows, max_rows, max_ctx, q, q_stride, out, n_heads, d_workspace,
+                                       workspace_bytes, (hipStream_t)stream},
+                                      what);
     if (p.bytes) {
         if (!d_workspace || workspace_bytes < p.bytes)
             return set_error(NYION_ERR_WORKSPACE, "%s: workspace %zu bytes < required %zu", what,

@@ -100,6 +100,58 @@ def test_prefill_options(gpu, code, options):
     check_prefill(gpu, code, (8, 4, 128), [(70, 200), (64, 64), (30, 300), (1, 5)], 32, **o)
 
 
+# Few rows per sequence: launches whose (row, head) pairs the decode's kernel takes.
+FEW = [(4, 200), (3, 3), (1, 300), (0, 50), (4, 64), (2, 1000), (4, 5)]
+
+
+@pytest.mark.parametrize("code", [E4M3, INT8])
+@pytest.mark.parametrize("shape,most", [((16, 4, 128), 4), ((8, 2, 64), 4), ((5, 1, 64), 3), ((21, 3, 128), 2),
+                                        ((4, 4, 64), 4), ((32, 2, 64), 4), ((15, 1, 128), 4), ((17, 1, 64), 1)])
+def test_prefill_of_few_rows(gpu, code, shape, most):
+    seqs = [(min(r, most), c) for r, c in FEW]
+    check_prefill(gpu, code, shape, seqs, 16)
+    check_prefill(gpu, code, shape, seqs, 64, strided=True, pad=len(seqs) * most - sum(r for r, _ in seqs),
+                  max_rows=most)
+    check_prefill(gpu, code, shape, [(most, 4000)], 32)
+
+
+@pytest.mark.parametrize("code", [E4M3, INT8])
+@pytest.mark.parametrize("options", [
+    dict(softcap=30.0), dict(softcap=0.5, q_scale=30.0), dict(slopes=True), dict(slopes=True, softcap=20.0),
+    dict(window=1), dict(window=3), dict(window=64), dict(window=100, slopes=True), dict(window=2 ** 31 - 1),
+    dict(scale=0.37), dict(prefix=[70, 0, 300, 5, 64, 998, 9]), dict(prefix=[200, 1000, 64, 1, 61, 0, 3], window=40),
+    dict(prefix=[199, 30, 300, 5, 62, 500, 4], slopes=True), dict(drop=[(0, -1), (2, 1 << 20)])])
+def test_prefill_of_few_rows_options(gpu, code, options):
+    o = dict(options)
+    if o.get("slopes"):
+        o["slopes"] = 2.0 ** (-8.0 * np.arange(1, 9) / 8)
+    check_prefill(gpu, code, (8, 2, 64), FEW, 16, **o)      # 16 pairs
+    check_prefill(gpu, code, (8, 1, 128), FEW, 32, **o)     # 32
+
+
+def test_prefill_of_few_rows_of_many_sequences(gpu):
+    rng = np.random.default_rng(70)
+    for n, shape in ((70, (8, 2, 64)), (1100, (2, 1, 64))):
+        check_prefill(gpu, E4M3, shape, [(int(r), int(r + c)) for r, c in zip(rng.integers(0, 5, n), rng.integers(0, 90, n))],
+                      16, max_rows=4)
+
+
+def test_prefill_of_few_rows_keeps_nan_to_its_row(gpu):
+    rng = np.random.default_rng(71)
+    codes, scales, tables = laid_out(rng, E4M3, [700], 2, 16, 64)
+    cache, q = gpu_cache(gpu, codes, scales, E4M3), torch.randn(4, 8, 64, device="cuda").bfloat16()
+    call = lambda q: gpu.kv8_prefill_bf16(cache, q, dev(tables), dev(np.array([700], np.int32)),  # noqa: E731
+                                          dev(np.array([0, 4], np.int32)), out)
+    out = torch.empty_like(q)
+    call(q)
+    want = out.clone()
+    q[1, 3, 5], q[2, 6, 0] = float("nan"), float("inf")
+    call(q)
+    assert out[1, 3].isnan().all() and out[2, 6].isnan().all()
+    out[1, 3], out[2, 6] = want[1, 3], want[2, 6]
+    assert torch.equal(out, want)
+
+
 @pytest.mark.parametrize("code,softcap", [(E4M3, 0.0), (INT8, 20.0)])
 @pytest.mark.parametrize("shape", [(2, 1, 64), (2, 2, 128)])
 def test_prefill_of_biased_rows_within_prefixes(gpu, code, softcap, shape):
