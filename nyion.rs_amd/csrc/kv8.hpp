@@ -73,6 +73,28 @@ __device__ __forceinline__ int kv8_block(const Kv8& c, const int32_t* table, int
     return (unsigned)b < (unsigned)c.num_blocks ? b : -1;
 }
 
+// The rows of sequence b of a ragged batch, and how far its keys go.
+struct Kv8Rows {
+    int row0, rows;  // of those that q holds
+    int pos0;        // position of row0
+    int live;        // its keys that can be read
+    int prefix;
+    __device__ __forceinline__ int key_end(int pos) const {  // of a row at pos, exclusive
+        return pos < 0 ? 0 : min(max(pos + 1, prefix), live);
+    }
+};
+__device__ __forceinline__ Kv8Rows kv8_rows(const int32_t* row_starts, const int32_t* ctx_lens,
+                                            const int32_t* prefix_lens, int n_rows, int span, int b) {
+    Kv8Rows s;
+    const int end = row_starts[b + 1], ctx = ctx_lens[b];
+    s.row0 = min(max(row_starts[b], 0), n_rows);
+    s.rows = min(max(end, s.row0), n_rows) - s.row0;
+    s.pos0 = (int)((unsigned)ctx - (unsigned)end + (unsigned)s.row0);
+    s.live = max(min(ctx, span), 0);
+    s.prefix = prefix_lens ? prefix_lens[b] : 0;
+    return s;
+}
+
 // Byte offset of kv head h of a block: 64 bits, a cache may pass 4 GiB.
 __device__ __forceinline__ long long kv8_offset(const Kv8& c, int block, int h) {
     return ((long long)block * c.n_kv_heads + h) * ((long long)c.head_dim << c.bt_log2);

@@ -150,25 +150,9 @@ __device__ __forceinline__ Kv8Span kv8_span(const Kv8DecodeArgs& a, int ctx) {
 }
 
 // The same for a sequence of several rows: the keys that any of them sees.
-struct Kv8Rows {
-    int row0, rows, pos0, live, prefix;
-};
-__device__ __forceinline__ Kv8Rows kv8_rows(const Kv8DecodeArgs& a, int b) {
-    Kv8Rows s;
-    const int end = a.row_starts[b + 1], ctx = a.ctx_lens[b];
-    s.row0 = min(max(a.row_starts[b], 0), a.n_rows);
-    s.rows = min(max(end, s.row0), a.n_rows) - s.row0;
-    s.pos0 = (int)((unsigned)ctx - (unsigned)end + (unsigned)s.row0);
-    s.live = max(min(ctx, a.span), 0);
-    s.prefix = a.s.prefix_lens ? a.s.prefix_lens[b] : 0;
-    return s;
-}
-__device__ __forceinline__ int key_end(const Kv8Rows& s, int pos) {
-    return pos < 0 ? 0 : min(max(pos + 1, s.prefix), s.live);
-}
 __device__ __forceinline__ Kv8Span kv8_span(const Kv8DecodeArgs& a, const Kv8Rows& s) {
     Kv8Span r;
-    r.hi = s.rows > 0 ? key_end(s, s.pos0 + s.rows - 1) : 0;
+    r.hi = s.rows > 0 ? s.key_end(s.pos0 + s.rows - 1) : 0;
     r.lo = a.s.window > 0 ? min(max(s.pos0 - a.s.window + 1, 0), r.hi) : 0;
     r.first = r.lo / kTile;
     r.tiles = max((int)(((unsigned)r.hi + kTile - 1) / kTile) - r.first, 1);
@@ -198,9 +182,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_decode_kernel(Kv8DecodeArg
     const int n = lane & 15;   // head of the group / row of an A operand
     const int g = lane >> 4;   // lane group
     const int units = a.c.n_kv_heads * a.n_hg;
+    const auto rows_of = [&](int b) {
+        return kv8_rows(a.row_starts, a.ctx_lens, a.s.prefix_lens, a.n_rows, a.span, b);
+    };
     const auto span_of = [&](int b, int ctx) {
         if constexpr (ROWS)
-            return kv8_span(a, kv8_rows(a, b));
+            return kv8_span(a, rows_of(b));
         else
             return kv8_span(a, ctx);
     };
@@ -362,7 +349,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_decode_kernel(Kv8DecodeArg
         int row0 = 0, i = 0, mine = n;  // ROWS: the sequence's first row, this lane's of it, its head of the group
         int key_lo, key_hi, all_lo, all_hi;  // ROWS: what this lane's pair sees, what all pairs see
         if constexpr (ROWS) {
-            const Kv8Rows rows = kv8_rows(a, b);
+            const Kv8Rows rows = rows_of(b);
             const int x0 = hg * 16;
             row0 = rows.row0;
             heads = max(min(16, rows.rows * a.group - x0), 0);
@@ -371,8 +358,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_decode_kernel(Kv8DecodeArg
             mine = x - i * a.group;
             const int first_pos = rows.pos0 + x0 / a.group, last_pos = rows.pos0 + (x0 + last) / a.group;
             qpos = rows.pos0 + i;
-            key_hi = key_end(rows, qpos);
-            all_hi = key_end(rows, first_pos);
+            key_hi = rows.key_end(qpos);
+            all_hi = rows.key_end(first_pos);
             key_lo = a.s.window > 0 ? max(qpos - a.s.window + 1, 0) : 0;
             all_lo = a.s.window > 0 ? max(last_pos - a.s.window + 1, 0) : 0;
         }

@@ -111,28 +111,11 @@ __device__ __forceinline__ float sum_half(float v) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// A sequence's rows and lengths.
-struct Rows {
-    int row0, rows;  // of those that q holds
-    int pos0;        // position of row0
-    int live, prefix;
-};
-__device__ __forceinline__ Rows rows_of(const Kv8PrefillArgs& a, int b) {
-    Rows s;
-    const int end = a.row_starts[b + 1], ctx = a.ctx_lens[b];
-    s.row0 = min(max(a.row_starts[b], 0), a.n_rows);
-    s.rows = min(max(end, s.row0), a.n_rows) - s.row0;
-    s.pos0 = (int)((unsigned)ctx - (unsigned)end + (unsigned)s.row0);
-    s.live = max(min(ctx, a.span), 0);
-    s.prefix = a.s.prefix_lens ? a.s.prefix_lens[b] : 0;
-    return s;
-}
-
 // The keys that a tile of pairs sees, as tiles of kKeys.
 struct PairSpan {
     int tile0, tiles;
 };
-__device__ __forceinline__ PairSpan pair_span(const Kv8PrefillArgs& a, const Rows& s, int tile, int tm) {
+__device__ __forceinline__ PairSpan pair_span(const Kv8PrefillArgs& a, const Kv8Rows& s, int tile, int tm) {
     PairSpan r;
     const int last_pair = min(tile * tm + tm, s.rows * a.group) - 1;
     const int first = s.pos0 + tile * tm / a.group, last = s.pos0 + last_pair / a.group;
@@ -154,7 +137,7 @@ kv8_prefill_kernel(Kv8PrefillArgs a) {
     constexpr int TM = kWavePairs * WAVES;  // (row, head) pairs per workgroup
     // per thread, of a tile's D * 4 K chunks of 16 bytes and V units of 4 tokens by 4 dims
     constexpr int KL = 4 * D / NT, VL = KL;
-    static_assert((kSeqsMax * (1 + sizeof(Rows) / 4) + kSorted) * 4 <= L::TILES, "the selection's lists");
+    static_assert((kSeqsMax * (1 + sizeof(Kv8Rows) / 4) + kSorted) * 4 <= L::TILES, "the selection's lists");
     static_assert(KL * NT == 4 * D, "every thread stages the same");
     __shared__ __attribute__((aligned(16))) unsigned char lds[L::BYTES];
     long long* const sub_off = (long long*)(lds + L::OFF);
@@ -174,16 +157,17 @@ kv8_prefill_kernel(Kv8PrefillArgs a) {
     int b = 0, tile = 0, kvh = 0, piece = 0;
     int item;
     PairSpan sp;
-    Rows seq;
+    Kv8Rows seq;
     {
         int* const ends = (int*)lds;  // tiles up to and with each sequence
-        Rows* const seqs = (Rows*)(ends + kSeqsMax);
+        Kv8Rows* const seqs = (Kv8Rows*)(ends + kSeqsMax);
         int before = 0;
         for (int b0 = 0; b0 < a.batch; b0 += NT) {
             const int s = b0 + tid;
             int x = 0;
             if (s < a.batch) {
-                const Rows mine = rows_of(a, s);
+                const Kv8Rows mine =
+                    kv8_rows(a.row_starts, a.ctx_lens, a.s.prefix_lens, a.n_rows, a.span, s);
                 seqs[s] = mine;
                 x = (int)(((long long)mine.rows * a.group + TM - 1) / TM);
             }

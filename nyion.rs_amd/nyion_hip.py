@@ -708,8 +708,9 @@ class ScoreOptions:
             _check_packed(torch.float32, slopes.get_device(), slopes)
         if prefix_lens is not None:
             _check_packed(torch.int32, prefix_lens.get_device(), prefix_lens)
-        self.slopes, self.prefix_lens, self.window = slopes, prefix_lens, window
-        self.struct = ScoreOptionsStruct(scale, softcap, window, 0, ptr(slopes), ptr(prefix_lens))
+        _want(window < 1 << 31, f"window {window} leaves 32 bits")
+        self.slopes, self.prefix_lens, self.window = slopes, prefix_lens, max(window, 0)
+        self.struct = ScoreOptionsStruct(scale, softcap, self.window, 0, ptr(slopes), ptr(prefix_lens))
         self.ref = C.addressof(self.struct)
 
     def check(self, n_heads, batch, device) -> None:

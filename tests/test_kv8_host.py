@@ -93,7 +93,7 @@ def test_handles_check_their_tensors():
             nh.Kv8Cache(*bad)
         assert e.value.code == nh.ERR_INVALID
     for bad in (dict(slopes=torch.zeros(8, dtype=torch.float64)), dict(slopes=torch.zeros(16)[::2]),
-                dict(prefix_lens=torch.zeros(8))):
+                dict(prefix_lens=torch.zeros(8)), dict(window=1 << 31), dict(window=(1 << 32) + 5)):
         with pytest.raises(nh.NyionError) as e:
             nh.ScoreOptions(**bad)
         assert e.value.code == nh.ERR_INVALID

@@ -302,6 +302,7 @@ def test_calls_of_many_shapes_take_turns_in_one_workspace(gpu):
         check_decode(gpu, E4M3, list(range(1, 2000, 40)), 4, 4, 16, 64, workspace=ws)
         check_prefill(gpu, INT8, (4, 1, 128), [(33, 1500), (0, 40), (5, 900 + i)], 16, workspace=ws)
         check_decode(gpu, E4M3, [2500, 900], 32, 1, 64, 128, io="bf16", workspace=ws)
+        check_prefill(gpu, E4M3, (8, 2, 64), [(2, 2900 + i), (1, 40), (4, 1000)], 32, workspace=ws)
     assert not ws[:16384].any()
 
 
@@ -386,6 +387,27 @@ def test_a_captured_step_serves_other_batches(gpu):
         assert (eager["ctx"].cpu().numpy() == lens).all() and int(eager["counts"][1]) == rows
         assert (eager["out"][rows:] == -7.0).all() and eager["out"][:rows].isfinite().all()
         left = left[int(eager["counts"][0]):]
+
+
+def test_prefill_of_few_rows_in_graphs(gpu):
+    rng = np.random.default_rng(72)
+    codes, scales, tables = laid_out(rng, E4M3, [3000, 500, 900], 2, 16, 64)
+    cache, q = gpu_cache(gpu, codes, scales, E4M3), torch.randn(12, 8, 64, device="cuda").bfloat16()
+    dlens, starts = dev(np.array([3000, 500, 900], np.int32)), dev(np.array([0, 4, 5, 9], np.int32))
+    tables, out, eager = dev(tables), torch.zeros_like(q), torch.zeros_like(q)
+    ws, graph = gpu.alloc_workspace(gpu.kv8_prefill_workspace_size(cache, 3, 8, 12, 4, 3000)), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        gpu.kv8_prefill_bf16(cache, q, tables, dlens, starts, out, max_rows=4, max_ctx=3000, workspace=ws)
+    for step, rows in enumerate(([4, 1, 4], [4, 4, 4], [0, 2, 3], [1, 1, 1])):
+        dlens.copy_(torch.tensor([3000 - 700 * step, 500 - step, 900 - 13 * step], dtype=torch.int32))
+        starts.copy_(dev(np.concatenate(([0], np.cumsum(rows))).astype(np.int32)))
+        q.copy_(torch.randn(12, 8, 64).bfloat16())
+        out.fill_(-7.0), eager.fill_(-7.0)
+        gpu.kv8_prefill_bf16(cache, q, tables, dlens, starts, eager, max_rows=4, max_ctx=3000)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager) and eager.isfinite().all(), step
+        assert (out[sum(rows):] == -7.0).all() and not (out[:sum(rows)] == -7.0).all()
 
 
 def rng_blocks(n):
